@@ -371,6 +371,102 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
                 float* lse, const int64_t* kv_lens, kuiops_stream_t stream);
 
 /* ======================================================================== */
+/* A KV cache across decode steps: trees of drafted tokens, bounded size    */
+/* ======================================================================== */
+#define KUIOPS_TREE_MAX_ROWS 4096u
+
+/* Attention of l drafted tokens (a tree, or any set of candidate continuations) over a cache plus their own
+ * keys and values, which are not in the cache yet: row i of batch entry b sees the cache keys j < kv_lens[b]
+ * (int64 on the device, clamped to [0, s]; NULL: all s) and the drafted keys j with mask[b, i, j] != 0, and
+ *     out_i = softmax(scale * q_i K^T) V,   lse_i = natural log-sum-exp (fp32, (n, h, l), may be NULL).
+ * Q is (n, h, l, e), the cache K / V (n, h_kv, s, e) / (n, h_kv, s, ev), DK / DV (n, h_kv, l, e) / (n, h_kv, l, ev),
+ * out (n, h, l, ev); element strides for (batch, head, row), innermost dimension contiguous; Q, DK and DV may be
+ * views of the packed projection rows kuiops_rope_qkv leaves.  mask is bytes, l x l per entry, mask_sn bytes
+ * from one entry to the next (0: one mask for all).  A key that a row does not see takes no part in it, whatever its
+ * rows hold (infinities, NaN); a row that sees no key gives 0 and -inf.  fp32 accumulation; 16-bit types round the
+ * softmax weights to the element type before the product with V, as kuiops_sdpa does.
+ * s may be 0 (K and V may then be NULL).  e <= 1024, ev <= 256 (KUIOPS_EUNSUPPORTED beyond),
+ * l <= KUIOPS_TREE_MAX_ROWS.  workspace: kuiops_sdpa_tree_workspace_bytes(...) bytes, 16-byte aligned, no initial
+ * contents required; calls that may overlap on the GPU need workspaces of their own.  No counterpart in the reference. */
+KUIOPS_API size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
+                                   uint32_t l, uint32_t s, uint32_t e, uint32_t ev);
+KUIOPS_API int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
+                uint32_t l, uint32_t s, uint32_t e, uint32_t ev,
+                const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
+                const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                const void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
+                const int64_t* kv_lens,
+                const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
+                const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
+                const void* mask, int64_t mask_sn, float scale,
+                void* out, int64_t o_sn, int64_t o_sh, int64_t o_sl, float* lse,
+                void* workspace, size_t workspace_bytes, kuiops_stream_t stream);
+
+/* Greedy acceptance of a verified tree.  parents is [l] int64 per sequence (parents_sn elements from one sequence to
+ * the next, 0: one tree for all): parents[0] = -1 (the root is the token that is certain), parents[i] < i, and -1
+ * for i > 0 marks a node that takes no part (padding).  draft is [n, l], the tokens of the nodes; target is [n, l], the
+ * model's token after each node.  A node is accepted when its parent is and draft[i] == target[parents[i]]; of the
+ * accepted nodes the deepest is chosen (equal depth: the lowest index).  path is [n, l]: the nodes from the root to it,
+ * then -1; counts[n] their number (at least 1); next[n] = target of the chosen node.  A parent that does not come before
+ * its node stores 1 in *status (which may be NULL) and the node is not accepted.  l <= KUIOPS_TREE_MAX_ROWS.
+ * No counterpart in the reference. */
+KUIOPS_API int kuiops_tree_accept(uint32_t n, uint32_t l, const int64_t* parents, int64_t parents_sn,
+                const int64_t* draft, const int64_t* target, int64_t* path, int64_t* counts, int64_t* next,
+                int32_t* status, kuiops_stream_t stream);
+
+/* Commits rows of DK / DV (n, h_kv, l, e | ev) to the caches K / V (n, h_kv, cap, e | ev): for t < counts[g] (all l when
+ * counts is NULL) row path[g, t] (row t when path is NULL) goes to slot kv_lens[g] + t, where entry b uses
+ * g = b % lens_n, so that one call serves every layer of a model (n = layers * lens_n).  When given, pos (n, h_kv, cap)
+ * receives next_pos[g] + t and mass (n, h_kv, cap) receives 0 at that slot.  lens_out[g] (may be NULL) =
+ * kv_lens[g] + counts[g], at most cap; kv_lens itself is not written, and the call may be repeated.  Elements of
+ * 1, 2 or 4 bytes.  A row or slot out of range is skipped and stores 1 in *status (which may be NULL).  No counterpart
+ * in the reference (its caches grow by cat, kuiops/cat/wrapper_cat.cu.j2:28-34). */
+KUIOPS_API int kuiops_kv_append(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t l, uint32_t cap, uint32_t e, uint32_t ev,
+                const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
+                const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
+                void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
+                const int64_t* kv_lens, uint32_t lens_n, const int64_t* path, const int64_t* counts,
+                int32_t* pos, const int64_t* next_pos, float* mass, int64_t* lens_out,
+                int32_t* status, kuiops_stream_t stream);
+
+/* The attention weight each key has received: for every slot j < s of every KV head
+ *     out[b, kh, j] = mass[b, kh, j] + sum over the query heads of kh and the rows i with j < lim_i of
+ *                     exp(scale * q_i . k_j - lse_i)
+ * with lse (n, h, l) from the attention call that ran before.  lim_i = q_lens[g, i] when q_lens is given ([lens_n, l],
+ * g = b % lens_n; at most kv_lens), else i + 1 + kv_lens[g] - l when is_causal (the alignment of kuiops_sdpa), else
+ * kv_lens[g] (NULL: s).  A row whose lse is infinite is not counted: -inf saw nothing, and a caller sets +inf to leave
+ * a row out.  mass == NULL counts as zeros; mass may be out.  Slots at or beyond kv_lens[g] keep their mass.
+ * Q (n, h, l, e) and K (n, h_kv, s, e) as in kuiops_sdpa; mass and out are dense (n, h_kv, s) fp32.  fp32 accumulation in a
+ * fixed order.  e <= 1024 (KUIOPS_EUNSUPPORTED beyond).  No counterpart in the reference. */
+KUIOPS_API int kuiops_attn_mass(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
+                const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
+                const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                const float* lse, const int64_t* kv_lens, uint32_t lens_n, const int64_t* q_lens,
+                float scale, int is_causal, const float* mass, float* out, kuiops_stream_t stream);
+
+/* Keeps `budget` of the kv_lens[g] slots of every (batch, KV head) row of a cache (g = b % lens_n): first the protected
+ * ones (0 <= pos < sinks, or pos >= next_pos[g] - recent), then those with the largest mass (NaN above +inf, as
+ * kuiops_topk_f32 orders them), equal ones by ascending slot.  The kept slots are not repacked: the i-th evicted slot
+ * below budget takes over the i-th kept slot at or above it, so attention over the first lens_out[g] =
+ * min(kv_lens[g], budget) slots sees the kept keys, in another order.  K and V rows move in place; rows at or beyond
+ * lens_out[g] stay as they were.  src (n, h_kv, budget) int32 = the slot each slot below budget came from (-1 beyond
+ * lens_out); mass_out and pos_out (n, h_kv, cap) = the kept slots' mass and positions, then 0 and -1.  pos is
+ * (n, h_kv, cap) int32, the token position of each slot; NULL: its slot; next_pos NULL: kv_lens.  A row with
+ * kv_lens[g] <= budget keeps everything.  The inputs mass, pos and kv_lens are not written (and must not be the
+ * outputs), so the call may be repeated.  1 <= budget <= cap, sinks + recent <= budget.  Elements of 1, 2 or 4 bytes.
+ * workspace: kuiops_kv_evict_workspace_bytes(...) bytes, 4-byte aligned, no initial contents required.  No counterpart
+ * in the reference. */
+KUIOPS_API size_t kuiops_kv_evict_workspace_bytes(uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t budget);
+KUIOPS_API int kuiops_kv_evict(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t e, uint32_t ev,
+                void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
+                const float* mass, const int32_t* pos, const int64_t* kv_lens, const int64_t* next_pos, uint32_t lens_n,
+                uint32_t budget, uint32_t sinks, uint32_t recent,
+                float* mass_out, int32_t* pos_out, int32_t* src, int64_t* lens_out,
+                void* workspace, size_t workspace_bytes, kuiops_stream_t stream);
+
+/* ======================================================================== */
 /* Streaming reductions                                                     */
 /* ======================================================================== */
 

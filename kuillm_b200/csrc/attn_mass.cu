@@ -1,0 +1,137 @@
+// The attention weight every key of a cache receives from a block of query rows, added up over the rows and over the
+// heads that share the key:
+//   out[b, kh, j] = mass[b, kh, j] + sum_{heads of kh} sum_{i: j < lim_i} exp(scale q_i . k_j - lse_i)
+// with lse from the attention call that ran before.  Softmax weights need the final row sums, so they cannot leave the
+// attention kernel in its one pass over the keys; this second pass reads K alone (no V) and needs no maximum.
+//
+// A key's sum is made by one thread in row order: no atomics, the result does not depend on timing.
+#include "tree.cuh"
+
+namespace kuiops {
+
+constexpr float kMassLog2e = 1.4426950408889634f;
+constexpr int kMassRows = 16;                    // query rows staged at a time
+
+// Keys of entry b that row li counts for.
+__device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, uint32_t li, uint32_t S) {
+  if (p.q_lens) return clamp_len(p.q_lens[size_t(b % p.lens_n) * p.l + li], S);
+  if (!p.is_causal) return S;
+  return clamp_len((long long)li + 1 + (long long)S - (long long)p.l, S);
+}
+
+// SIMT form for every type, head dimension and stride: a thread owns a key, whose row it keeps in shared memory (rows
+// padded to an odd length: no bank conflicts), and dots it with sixteen query rows at a time, broadcast from shared
+// memory.  fp32 arithmetic throughout.
+template <typename T>
+__global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
+  extern __shared__ __align__(16) float sm[];
+  const uint32_t KT = blockDim.x, ep = p.e | 1u, e4 = (p.e + 3) & ~3u;
+  float* q_s = sm;                               // [kMassRows][e4]
+  float* lse_s = q_s + kMassRows * e4;
+  uint32_t* lim_s = reinterpret_cast<uint32_t*>(lse_s + kMassRows);
+  float* k_s = reinterpret_cast<float*>(lim_s + kMassRows);     // [KT][ep]
+  const uint32_t kt = blockIdx.x % key_tiles, u = blockIdx.x / key_tiles, kvh = u % p.h_kv, b = u / p.h_kv;
+  const uint32_t G = p.h / p.h_kv, rows = G * p.l, key0 = kt * KT, j = key0 + threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t S = p.kv_lens ? clamp_len(p.kv_lens[b % p.lens_n], p.s) : p.s;
+  float total = 0.f;
+  if (key0 < S) {
+    const T* Kb = static_cast<const T*>(p.K) + int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh;
+    const uint32_t nk = min(KT, S - key0);
+    for (uint32_t i = threadIdx.x; i < nk * p.e; i += KT)
+      k_s[(i / p.e) * ep + i % p.e] = ElemTraits<T>::to_f(Kb[int64_t(key0 + i / p.e) * p.k_ss + i % p.e]);
+    const float* krow = k_s + threadIdx.x * ep;
+    const float qmul = p.scale * kMassLog2e;
+    for (uint32_t r0 = 0; r0 < rows; r0 += kMassRows) {
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < kMassRows * e4; i += KT) {
+        const uint32_t row = r0 + i / e4, c = i % e4;
+        q_s[i] = row < rows && c < p.e ? ElemTraits<T>::to_f(static_cast<const T*>(p.Q)[int64_t(b) * p.q_sn +
+                     int64_t(kvh * G + row / p.l) * p.q_sh + int64_t(row % p.l) * p.q_sl + c]) : 0.f;
+      }
+      for (uint32_t i = threadIdx.x; i < kMassRows; i += KT) {
+        const uint32_t row = r0 + i;
+        float ls = INFINITY;
+        uint32_t lim = 0;
+        if (row < rows) {
+          ls = p.lse[(size_t(b) * p.h + kvh * G + row / p.l) * p.l + row % p.l];
+          // a row that saw nothing (-inf) or is not to be counted (+inf) has no weight to give
+          if (!isinf(ls)) lim = mass_limit(p, b, row % p.l, S);
+        }
+        lse_s[i] = ls * kMassLog2e;
+        lim_s[i] = lim;
+      }
+      __syncthreads();
+      if (j < S) {
+        float sc[kMassRows];
+#pragma unroll
+        for (int r = 0; r < kMassRows; ++r) sc[r] = 0.f;
+        for (uint32_t c = 0; c < p.e; ++c) {
+          const float kf = krow[c];
+#pragma unroll
+          for (int r = 0; r < kMassRows; ++r) sc[r] = fmaf(q_s[r * e4 + c], kf, sc[r]);
+        }
+        float part = 0.f;
+#pragma unroll
+        for (int r = 0; r < kMassRows; ++r)
+          if (j < lim_s[r]) part += exp2f(fmaf(sc[r], qmul, -lse_s[r]));
+        total += part;
+      }
+    }
+  }
+  if (j < p.s) {
+    const size_t o = (size_t(b) * p.h_kv + kvh) * p.s + j;
+    p.out[o] = (p.mass ? p.mass[o] : 0.f) + total;
+  }
+}
+
+template <typename T>
+static int mass_simt_launch(const MassArgs& a, cudaStream_t st) {
+  // a CTA's key rows have to fit shared memory: 128 keys of up to 256 features, 32 of up to 1024
+  const uint32_t KT = a.e <= 256 ? 128 : 32, tiles = (a.s + KT - 1) / KT;
+  const size_t smem = (size_t(kMassRows) * (((a.e + 3) & ~3u) + 2) + size_t(KT) * (a.e | 1u)) * sizeof(float);
+  auto kern = attn_mass_simt_kernel<T>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    return KUIOPS_ELAUNCH;
+  const uint64_t grid = uint64_t(a.n) * a.h_kv * tiles;
+  if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
+  return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT), smem, st, a, tiles);
+}
+
+int attn_mass_simt(const MassArgs& a, cudaStream_t st) {
+  switch (a.dtype) {
+    case KUIOPS_F32: return mass_simt_launch<float>(a, st);
+    case KUIOPS_BF16: return mass_simt_launch<__nv_bfloat16>(a, st);
+    default: return mass_simt_launch<__half>(a, st);
+  }
+}
+
+}  // namespace kuiops
+
+using namespace kuiops;
+
+extern "C" {
+
+int kuiops_attn_mass(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
+                     const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
+                     const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                     const float* lse, const int64_t* kv_lens, uint32_t lens_n, const int64_t* q_lens,
+                     float scale, int is_causal, const float* mass, float* out, kuiops_stream_t stream) {
+  if (dtype != KUIOPS_F32 && dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_EINVAL;
+  if (n == 0 || h == 0 || h_kv == 0 || l == 0 || s == 0 || e == 0 || h % h_kv) return KUIOPS_EINVAL;
+  if (!Q || !K || !lse || !out || q_sl < int64_t(e) || k_ss < int64_t(e)) return KUIOPS_EINVAL;
+  if ((kv_lens || q_lens) && (lens_n == 0 || n % lens_n)) return KUIOPS_EINVAL;
+  if (!(scale - scale == 0.f)) return KUIOPS_EINVAL;
+  if (e > 1024) return KUIOPS_EUNSUPPORTED;
+  if (s > 0x7fffff00u || uint64_t(h / h_kv) * l >= (1ull << 31)) return KUIOPS_ELIMIT;
+  MassArgs a = {};
+  a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e;
+  a.Q = Q; a.q_sn = q_sn; a.q_sh = q_sh; a.q_sl = q_sl;
+  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
+  a.lse = lse; a.kv_lens = kv_lens; a.lens_n = lens_n ? lens_n : 1; a.q_lens = q_lens;
+  a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.mass = mass; a.out = out;
+  return attn_mass_simt(a, as_stream(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,322 @@
+// Attention of l drafted tokens over a KV cache plus their own keys under an l x l mask:
+//   out_i = sum_j w_ij v_j,   w_ij = exp(scale q_i . k_j - lse_i),   lse_i = log sum_j exp(scale q_i . k_j)
+// over the cache keys j < kv_lens[b] and the drafted keys j with mask[b, i, j] != 0.  A masked key takes no part
+// at all: whatever its row holds (infinities, NaN) reaches no output, and a row that sees nothing gives 0 / -inf.
+//
+// This file holds the entry point, the SIMT kernel for every type, head dimension and stride, and the kernel that
+// joins key slices.  16-bit operands with up to 128 features per head run on the tensor cores (sdpa_tree_tc.cu).
+#include "tree.cuh"
+
+namespace kuiops {
+
+constexpr float kTreeLog2e = 1.4426950408889634f;
+constexpr float kTreeLn2 = 0.6931471805599453f;
+
+// SIMT form: a CTA owns R query rows of one (batch, KV head) and a slice of the 32-key tiles (cache tiles first, then
+// the drafted ones).  Its four warps take tiles in turn; for the scores a lane owns a key and dots it with the R rows
+// in shared memory, for the values a lane owns DV columns.  All arithmetic in fp32, softmax online in the log2 domain.
+template <typename T, int R, int DV>
+__global__ void __launch_bounds__(128)
+sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32_t row_blocks, uint32_t e_pad) {
+  extern __shared__ __align__(16) float sm[];
+  constexpr int ACCW = DV * 32 + 2;
+  float* q_s = sm;                                  // [R][e_pad]
+  float* mrg = sm + R * e_pad;                      // [4 warps][R][ACCW]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t split = blockIdx.x % splits;
+  uint32_t u = blockIdx.x / splits;
+  const uint32_t rb = u % row_blocks; u /= row_blocks;
+  const uint32_t kvh = u % p.h_kv, b = u / p.h_kv;
+  const uint32_t G = p.h / p.h_kv, rows = G * p.l;  // row = (head in group) * l + position
+  pdl_wait();
+  pdl_trigger();
+
+  const float qmul = p.scale * kTreeLog2e;
+  for (uint32_t i = tid; i < R * e_pad; i += 128) {
+    const uint32_t row = rb * R + i / e_pad, c = i % e_pad;
+    float v = 0.f;
+    if (row < rows && c < p.e)
+      v = ElemTraits<T>::to_f(static_cast<const T*>(p.Q)[int64_t(b) * p.q_sn + int64_t(kvh * G + row / p.l) * p.q_sh +
+                                                         int64_t(row % p.l) * p.q_sl + c]);
+    q_s[i] = v;
+  }
+  __syncthreads();
+
+  const uint32_t S = p.kv_lens ? clamp_len(p.kv_lens[b], p.s) : p.s;
+  const uint32_t cache_tiles = (S + 31) / 32, tiles = cache_tiles + (p.l + 31) / 32;
+  const uint32_t per = (tiles + splits - 1) / splits;
+  const uint32_t t_lo = min(split * per, tiles), t_hi = min(t_lo + per, tiles);
+  const T* Kb = static_cast<const T*>(p.K) + int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh;
+  const T* Vb = static_cast<const T*>(p.V) + int64_t(b) * p.v_sn + int64_t(kvh) * p.v_sh;
+  const T* Kd = static_cast<const T*>(p.DK) + int64_t(b) * p.dk_sn + int64_t(kvh) * p.dk_sh;
+  const T* Vd = static_cast<const T*>(p.DV) + int64_t(b) * p.dv_sn + int64_t(kvh) * p.dv_sh;
+  const unsigned char* mk = p.mask + int64_t(b) * p.m_sn;
+
+  float m[R], lsum[R], acc[R][DV];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY; lsum[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) acc[r][d] = 0.f;
+  }
+
+  for (uint32_t t = t_lo + warp; t < t_hi; t += 4) {
+    const bool drafted = t >= cache_tiles;
+    const uint32_t key0 = drafted ? (t - cache_tiles) * 32 : t * 32;
+    const uint32_t limit = drafted ? p.l : S;
+    const uint32_t j = key0 + lane;
+    const bool inside = j < limit;
+    float sc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) sc[r] = 0.f;
+    if (inside) {
+      const T* krow = drafted ? Kd + int64_t(j) * p.dk_sl : Kb + int64_t(j) * p.k_ss;
+      uint32_t c = 0;
+      if ((reinterpret_cast<uintptr_t>(krow) & 15u) == 0) {
+        constexpr int N = Vec16<T>::N;
+        for (; c + N <= p.e; c += N) {
+          const Vec16<T> kv = ld16(krow + c);
+          float kf[N];
+#pragma unroll
+          for (int x = 0; x < N; ++x) kf[x] = ElemTraits<T>::to_f(kv.v[x]);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float* q = q_s + r * e_pad + c;
+#pragma unroll
+            for (int x = 0; x < N; ++x) sc[r] = fmaf(q[x], kf[x], sc[r]);
+          }
+        }
+      }
+      for (; c < p.e; ++c) {
+        const float kf = ElemTraits<T>::to_f(krow[c]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) sc[r] = fmaf(q_s[r * e_pad + c], kf, sc[r]);
+      }
+    }
+    float pr[R];
+    uint32_t vis[R];                                // keys of the tile that row r sees, one bit per key
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t row = rb * R + r;
+      bool v = inside && row < rows;
+      if (v && drafted) v = mk[size_t(row % p.l) * p.l + j] != 0;
+      vis[r] = __ballot_sync(0xffffffffu, v);
+      const float s2 = v ? sc[r] * qmul : -INFINITY;
+      const float mn = fmaxf(m[r], warp_max(s2));
+      float corr = 1.f, pv = 0.f;
+      if (mn != -INFINITY) corr = exp2f(m[r] - mn);            // m[r] = -inf gives 0
+      if (v) pv = exp2f(s2 - (mn == -INFINITY ? 0.f : mn));     // a NaN score stays one
+      lsum[r] = lsum[r] * corr + warp_sum(pv);
+      m[r] = mn;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) acc[r][d] *= corr;
+      pr[r] = pv;
+    }
+    uint32_t any = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) any |= vis[r];
+    const uint32_t d0 = lane * DV;
+    while (any) {
+      const int jj = __ffs(any) - 1;
+      any &= any - 1;
+      const T* vrow = drafted ? Vd + int64_t(key0 + jj) * p.dv_sl : Vb + int64_t(key0 + jj) * p.v_ss;
+      float vf[DV];
+#pragma unroll
+      for (int d = 0; d < DV; ++d) vf[d] = (d0 + d < p.ev) ? ElemTraits<T>::to_f(vrow[d0 + d]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float pj = __shfl_sync(0xffffffffu, pr[r], jj);
+        if ((vis[r] >> jj) & 1u) {
+#pragma unroll
+          for (int d = 0; d < DV; ++d) acc[r][d] = fmaf(pj, vf[d], acc[r][d]);
+        }
+      }
+    }
+  }
+
+  // join the four warps in warp order
+  {
+    float* mine = mrg + size_t(warp) * R * ACCW;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int d = 0; d < DV; ++d) mine[r * ACCW + lane * DV + d] = acc[r][d];
+      if (lane == 0) { mine[r * ACCW + DV * 32] = m[r]; mine[r * ACCW + DV * 32 + 1] = lsum[r]; }
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < R * p.ev; i += 128) {
+    const uint32_t r = i / p.ev, c = i % p.ev, row = rb * R + r;
+    if (row >= rows) continue;
+    float mm = -INFINITY;
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mrg[(w * R + r) * ACCW + DV * 32]);
+    float a = 0.f, den = 0.f;
+    for (int w = 0; w < 4; ++w) {
+      const float* rec = mrg + (w * R + r) * ACCW;
+      const float f = rec[DV * 32] == -INFINITY ? 0.f : exp2f(rec[DV * 32] - mm);
+      // a slice whose scores were all NaN has no maximum but a NaN sum: the product keeps it
+      a += f * rec[c]; den += f * rec[DV * 32 + 1];
+    }
+    const uint32_t head = kvh * G + row / p.l, li = row % p.l;
+    const uint64_t orow = (uint64_t(b) * p.h + head) * p.l + li;
+    if (splits == 1) {
+      static_cast<T*>(p.out)[int64_t(b) * p.o_sn + int64_t(head) * p.o_sh + int64_t(li) * p.o_sl + c] =
+          ElemTraits<T>::from_f(den == 0.f ? 0.f : a / den);
+      if (c == 0 && p.lse) p.lse[orow] = den == 0.f ? -INFINITY : (mm + log2f(den)) * kTreeLn2;
+    } else {
+      float* rec = tree_record(partials, orow, splits, split, p.ev);
+      rec[c] = a;
+      if (c == 0) { rec[tree_record_floats(p.ev) - 4] = mm; rec[tree_record_floats(p.ev) - 3] = den; }
+    }
+  }
+}
+
+// One warp per output row: the slices' records are added in slice order, so the result does not depend on timing.
+template <typename T>
+__global__ void __launch_bounds__(128)
+sdpa_tree_merge_kernel(const TreeArgs p, const float* partials, uint32_t splits) {
+  const uint64_t row = uint64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const uint32_t lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= uint64_t(p.n) * p.h * p.l) return;
+  const uint32_t rl = tree_record_floats(p.ev);
+  const float* base = partials + row * splits * rl;
+  float mm = -INFINITY;
+  for (uint32_t s = lane; s < splits; s += 32) mm = fmaxf(mm, __ldg(base + size_t(s) * rl + rl - 4));
+  mm = warp_max(mm);
+  const uint32_t li = uint32_t(row % p.l), head = uint32_t(row / p.l % p.h), b = uint32_t(row / (uint64_t(p.l) * p.h));
+  T* orow = static_cast<T*>(p.out) + int64_t(b) * p.o_sn + int64_t(head) * p.o_sh + int64_t(li) * p.o_sl;
+  float den = 0.f;
+  for (uint32_t c0 = 0; c0 < p.ev; c0 += 128) {
+    const uint32_t c = c0 + lane * 4;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    den = 0.f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < splits; ++s) {
+      const float* rec = base + size_t(s) * rl;
+      const float mw = __ldg(rec + rl - 4), lw = __ldg(rec + rl - 3);
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mm);
+      den += f * lw;
+      if (c < p.ev) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(rec + c));
+        acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (c + x < p.ev) orow[c + x] = ElemTraits<T>::from_f(den == 0.f ? 0.f : acc[x] / den);
+  }
+  if (p.lse && lane == 0) p.lse[row] = den == 0.f ? -INFINITY : (mm + log2f(den)) * kTreeLn2;
+}
+
+template <typename T, int R, int DV>
+static int simt_launch(const TreeArgs& a, float* partials, uint32_t splits, cudaStream_t st) {
+  const uint32_t e_pad = (a.e + 3) & ~3u, rows = a.h / a.h_kv * a.l, row_blocks = (rows + R - 1) / R;
+  const size_t smem = (size_t(R) * e_pad + size_t(4) * R * (DV * 32 + 2)) * sizeof(float);
+  auto kern = sdpa_tree_simt_kernel<T, R, DV>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    return KUIOPS_ELAUNCH;
+  const uint64_t grid = uint64_t(a.n) * a.h_kv * row_blocks * splits;
+  if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
+  return launch_pdl(kern, dim3(unsigned(grid)), dim3(128), smem, st, a, partials, splits, row_blocks, e_pad);
+}
+
+template <typename T>
+static int simt_launch_t(const TreeArgs& a, float* partials, uint32_t splits, cudaStream_t st) {
+  const bool few = a.h / a.h_kv * a.l <= 4;
+  if (a.ev <= 64) return few ? simt_launch<T, 4, 2>(a, partials, splits, st) : simt_launch<T, 8, 2>(a, partials, splits, st);
+  if (a.ev <= 128) return few ? simt_launch<T, 4, 4>(a, partials, splits, st) : simt_launch<T, 8, 4>(a, partials, splits, st);
+  return few ? simt_launch<T, 4, 8>(a, partials, splits, st) : simt_launch<T, 8, 8>(a, partials, splits, st);
+}
+
+// Slices per (batch, KV head, row block): as many CTAs as two waves hold (a 128-thread CTA, four to an SM), with at
+// least sixteen 32-key tiles each, so that joining stays small beside the keys read.
+uint32_t sdpa_tree_simt_splits(const TreeArgs& a) {
+  const uint32_t rows = a.h / a.h_kv * a.l, R = rows <= 4 ? 4 : 8;
+  const uint64_t units = uint64_t(a.n) * a.h_kv * ((rows + R - 1) / R), want = 8ull * num_sms() / units;
+  const uint32_t cap = (a.s / 32 + (a.l + 31) / 32) / 16;
+  const uint64_t v = want < cap ? want : cap;
+  return v < 1 ? 1u : (v > 64 ? 64u : uint32_t(v));
+}
+
+int sdpa_tree_simt(const TreeArgs& a, float* partials, uint32_t splits, cudaStream_t st) {
+  switch (a.dtype) {
+    case KUIOPS_F32: return simt_launch_t<float>(a, partials, splits, st);
+    case KUIOPS_BF16: return simt_launch_t<__nv_bfloat16>(a, partials, splits, st);
+    default: return simt_launch_t<__half>(a, partials, splits, st);
+  }
+}
+
+int sdpa_tree_merge(const TreeArgs& a, const float* partials, uint32_t splits, cudaStream_t st) {
+  const uint64_t grid = (uint64_t(a.n) * a.h * a.l + 3) / 4;
+  if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
+  switch (a.dtype) {
+    case KUIOPS_F32: return launch_pdl(sdpa_tree_merge_kernel<float>, dim3(unsigned(grid)), dim3(128), 0, st, a, partials, splits);
+    case KUIOPS_BF16: return launch_pdl(sdpa_tree_merge_kernel<__nv_bfloat16>, dim3(unsigned(grid)), dim3(128), 0, st, a, partials, splits);
+    default: return launch_pdl(sdpa_tree_merge_kernel<__half>, dim3(unsigned(grid)), dim3(128), 0, st, a, partials, splits);
+  }
+}
+
+}  // namespace kuiops
+
+using namespace kuiops;
+
+static int tree_shape(TreeArgs& a, int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev) {
+  if (dtype != KUIOPS_F32 && dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_EINVAL;
+  if (n == 0 || h == 0 || h_kv == 0 || l == 0 || e == 0 || ev == 0 || h % h_kv) return KUIOPS_EINVAL;
+  if (e > 1024 || ev > 256) return KUIOPS_EUNSUPPORTED;
+  if (l > KUIOPS_TREE_MAX_ROWS || s > 0x7fffff00u || uint64_t(n) * h * l >= (1ull << 31)) return KUIOPS_ELIMIT;
+  a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e; a.ev = ev;
+  return KUIOPS_OK;
+}
+
+static size_t tree_record_bytes(const TreeArgs& a, uint32_t splits) {
+  return splits <= 1 ? 0 : size_t(a.n) * a.h * a.l * splits * tree_record_floats(a.ev) * sizeof(float);
+}
+
+extern "C" {
+
+size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
+                                        uint32_t ev) {
+  TreeArgs a = {};
+  if (tree_shape(a, dtype, n, h, h_kv, l, s, e, ev) != KUIOPS_OK) return 0;
+  return tree_record_bytes(a, sdpa_tree_simt_splits(a));
+}
+
+int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev,
+                     const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
+                     const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
+                     const void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
+                     const int64_t* kv_lens,
+                     const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
+                     const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
+                     const void* mask, int64_t mask_sn, float scale,
+                     void* out, int64_t o_sn, int64_t o_sh, int64_t o_sl, float* lse,
+                     void* workspace, size_t workspace_bytes, kuiops_stream_t stream) {
+  TreeArgs a = {};
+  const int rc = tree_shape(a, dtype, n, h, h_kv, l, s, e, ev);
+  if (rc != KUIOPS_OK) return rc;
+  if (!Q || !DK || !DV || !mask || !out || (s > 0 && (!K || !V))) return KUIOPS_EINVAL;
+  if (q_sl < int64_t(e) || dk_sl < int64_t(e) || dv_sl < int64_t(ev) || o_sl < int64_t(ev)) return KUIOPS_EINVAL;
+  if (s > 0 && (k_ss < int64_t(e) || v_ss < int64_t(ev))) return KUIOPS_EINVAL;
+  if (mask_sn != 0 && mask_sn < int64_t(l) * l) return KUIOPS_EINVAL;
+  if (!(scale - scale == 0.f)) return KUIOPS_EINVAL;              // a finite number
+  a.Q = Q; a.q_sn = q_sn; a.q_sh = q_sh; a.q_sl = q_sl;
+  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
+  a.V = V; a.v_sn = v_sn; a.v_sh = v_sh; a.v_ss = v_ss;
+  a.kv_lens = kv_lens;
+  a.DK = DK; a.dk_sn = dk_sn; a.dk_sh = dk_sh; a.dk_sl = dk_sl;
+  a.DV = DV; a.dv_sn = dv_sn; a.dv_sh = dv_sh; a.dv_sl = dv_sl;
+  a.mask = static_cast<const unsigned char*>(mask); a.m_sn = mask_sn;
+  a.scale = scale; a.out = out; a.o_sn = o_sn; a.o_sh = o_sh; a.o_sl = o_sl; a.lse = lse;
+  cudaStream_t st = as_stream(stream);
+  const uint32_t splits = sdpa_tree_simt_splits(a);
+  if (splits > 1 && (!workspace || workspace_bytes < tree_record_bytes(a, splits) || !aligned16(workspace))) return KUIOPS_EWORKSPACE;
+  float* partials = static_cast<float*>(workspace);
+  const int run = sdpa_tree_simt(a, partials, splits, st);
+  if (run != KUIOPS_OK || splits == 1) return run;
+  return sdpa_tree_merge(a, partials, splits, st);
+}
+
+}  // extern "C"

@@ -491,3 +491,92 @@ def sample_topk_topp(logits: np.ndarray, temperature: float, top_k: int, top_p: 
         d_pick = np.abs(incl_r[:R].astype(np.float64) - float(t)).min() / scale
         margin[r] = min(d_cut, d_pick)
     return ids.reshape(logits.shape[:-1]), prob.reshape(logits.shape[:-1]), margin.reshape(logits.shape[:-1])
+
+
+# --------------------------------------------------------------------------------------------
+# a KV cache across decode steps (64-bit definitions; none of these has a counterpart in the reference)
+# --------------------------------------------------------------------------------------------
+def sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, scale=None):
+    """(out, lse, sum of w |v|, largest sum of |q k| a score is made of) of attention over the first kv_lens[b] cache
+    keys and the drafted keys mask[b] lets a row see.  The last two size the error bounds of a finite-precision kernel."""
+    Q, K, V, Kd, Vd = (np.asarray(x, np.float64) for x in (Q, K, V, Kd, Vd))
+    n, h, l, e = Q.shape
+    g = h // K.shape[1]
+    scale = e ** -0.5 if scale is None else scale
+    out, mag = np.zeros((n, h, l, V.shape[3])), np.zeros((n, h, l, V.shape[3]))
+    lse, reach = np.full((n, h, l), -np.inf), 0.0
+    for b in range(n):
+        s = min(max(int(kv_lens[b]), 0), K.shape[2])
+        m = np.asarray(mask[b % len(mask)], bool)
+        for i in range(h):
+            for r in range(l):
+                keys = np.concatenate([K[b, i // g, :s], Kd[b, i // g][m[r]]])
+                vals = np.concatenate([V[b, i // g, :s], Vd[b, i // g][m[r]]])
+                if len(keys) == 0:
+                    continue
+                x = keys @ Q[b, i, r] * scale
+                if np.isfinite(x).all():
+                    reach = max(reach, float((np.abs(keys) @ np.abs(Q[b, i, r])).max()) * abs(scale))
+                with np.errstate(invalid="ignore"):
+                    w = np.exp(x - x.max())
+                    lse[b, i, r] = x.max() + np.log(w.sum())
+                    w = w / w.sum()
+                    out[b, i, r] = w @ vals
+                    mag[b, i, r] = w @ np.abs(vals)
+    return out, lse, mag, reach
+
+
+def tree_accept(parents, draft, target):
+    """(path, counts, next) of the greedy walk, one sequence after the other."""
+    n, l = draft.shape
+    path, counts, nxt = np.full((n, l), -1, np.int64), np.zeros(n, np.int64), np.zeros(n, np.int64)
+    for b in range(n):
+        par = parents[b % len(parents)]
+        chains = {0: [0]}
+        for i in range(1, l):
+            p = int(par[i])
+            if 0 <= p < i and p in chains and draft[b, i] == target[b, p]:
+                chains[i] = chains[p] + [i]
+        best = max(chains, key=lambda i: (len(chains[i]), -i))
+        path[b, :len(chains[best])] = chains[best]
+        counts[b], nxt[b] = len(chains[best]), target[b, best]
+    return path, counts, nxt
+
+
+def attn_mass(Q, K, lse, kv_lens, limits, mass, scale=None):
+    """(out, largest sum of |q k|): limits [n, l] = leading keys a row counts for."""
+    Q, K, lse = (np.asarray(x, np.float64) for x in (Q, K, lse))
+    n, h, l, e = Q.shape
+    hk, s = K.shape[1], K.shape[2]
+    g = h // hk
+    scale = e ** -0.5 if scale is None else scale
+    out, reach = np.array(mass, np.float64), 0.0
+    for b in range(n):
+        cap = min(max(int(kv_lens[b]), 0), s)
+        for i in range(h):
+            for r in range(l):
+                lim = min(max(int(limits[b][r]), 0), cap)
+                if lim == 0 or np.isinf(lse[b, i, r]):
+                    continue
+                k = K[b, i // g, :lim]
+                out[b, i // g, :lim] += np.exp(k @ Q[b, i, r] * scale - lse[b, i, r])
+                reach = max(reach, float((np.abs(k) @ np.abs(Q[b, i, r])).max()) * abs(scale))
+    return out, reach
+
+
+def kv_evict_map(mass, pos, length, next_pos, budget, sinks, recent):
+    """The slot map of one row: src[i] = the slot that slot i < min(length, budget) holds afterwards, by the definition
+    (protected first, larger mass, lower slot), decided with Python's exact comparisons."""
+    def order(j):
+        held = 0 <= pos[j] < sinks or pos[j] >= next_pos - recent
+        w = float(mass[j])
+        return (0 if held else 1, 0.0 if held else (-np.inf if w != w else 0.0), 0.0 if held or w != w else -w, j)
+    if length <= budget:
+        return list(range(length))
+    kept = set(sorted(range(length), key=order)[:budget])
+    holes = [j for j in range(budget) if j not in kept]
+    movers = [j for j in range(budget, length) if j in kept]
+    src = list(range(budget))
+    for to, frm in zip(holes, movers):
+        src[to] = frm
+    return src
