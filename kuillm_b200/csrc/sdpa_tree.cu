@@ -183,7 +183,7 @@ sdpa_tree_merge_kernel(const TreeArgs p, const float* partials, uint32_t splits)
   const uint32_t rl = tree_record_floats(p.ev);
   const float* base = partials + row * splits * rl;
   float mm = -INFINITY;
-  for (uint32_t s = lane; s < splits; s += 32) mm = fmaxf(mm, __ldg(base + size_t(s) * rl + rl - 4));
+  for (uint32_t s = lane; s < splits; s += 32) mm = fmaxf(mm, __ldcg(base + size_t(s) * rl + rl - 4));
   mm = warp_max(mm);
   const uint32_t li = uint32_t(row % p.l), head = uint32_t(row / p.l % p.h), b = uint32_t(row / (uint64_t(p.l) * p.h));
   T* orow = static_cast<T*>(p.out) + int64_t(b) * p.o_sn + int64_t(head) * p.o_sh + int64_t(li) * p.o_sl;
@@ -195,11 +195,11 @@ sdpa_tree_merge_kernel(const TreeArgs p, const float* partials, uint32_t splits)
 #pragma unroll 4
     for (uint32_t s = 0; s < splits; ++s) {
       const float* rec = base + size_t(s) * rl;
-      const float mw = __ldg(rec + rl - 4), lw = __ldg(rec + rl - 3);
+      const float mw = __ldcg(rec + rl - 4), lw = __ldcg(rec + rl - 3);
       const float f = mw == -INFINITY ? 0.f : exp2f(mw - mm);
       den += f * lw;
       if (c < p.ev) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(rec + c));
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + c));
         acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
       }
     }
@@ -281,7 +281,10 @@ size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint3
                                         uint32_t ev) {
   TreeArgs a = {};
   if (tree_shape(a, dtype, n, h, h_kv, l, s, e, ev) != KUIOPS_OK) return 0;
-  return tree_record_bytes(a, sdpa_tree_simt_splits(a));
+  // which kernel runs also depends on alignment, unknown here: cover both
+  const uint32_t simt = sdpa_tree_simt_splits(a);
+  const uint32_t tc = dtype != KUIOPS_F32 && e <= 128 && ev <= 128 && h / h_kv <= 128 ? sdpa_tree_tc_splits(a) : 1;
+  return tree_record_bytes(a, simt > tc ? simt : tc);
 }
 
 int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev,
@@ -311,10 +314,11 @@ int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t 
   a.mask = static_cast<const unsigned char*>(mask); a.m_sn = mask_sn;
   a.scale = scale; a.out = out; a.o_sn = o_sn; a.o_sh = o_sh; a.o_sl = o_sl; a.lse = lse;
   cudaStream_t st = as_stream(stream);
-  const uint32_t splits = sdpa_tree_simt_splits(a);
+  const bool tc = sdpa_tree_tc_eligible(a);
+  const uint32_t splits = tc ? sdpa_tree_tc_splits(a) : sdpa_tree_simt_splits(a);
   if (splits > 1 && (!workspace || workspace_bytes < tree_record_bytes(a, splits) || !aligned16(workspace))) return KUIOPS_EWORKSPACE;
   float* partials = static_cast<float*>(workspace);
-  const int run = sdpa_tree_simt(a, partials, splits, st);
+  const int run = tc ? sdpa_tree_tc(a, partials, st) : sdpa_tree_simt(a, partials, splits, st);
   if (run != KUIOPS_OK || splits == 1) return run;
   return sdpa_tree_merge(a, partials, splits, st);
 }

@@ -33,6 +33,11 @@ int sdpa_tree_simt(const TreeArgs& a, float* partials, uint32_t splits, cudaStre
 // Joins the records of `splits` slices into out / lse.
 int sdpa_tree_merge(const TreeArgs& a, const float* partials, uint32_t splits, cudaStream_t st);
 
+// The tensor-core kernel; sdpa_tree_tc_splits does not depend on pointers and strides.
+bool sdpa_tree_tc_eligible(const TreeArgs& a);
+uint32_t sdpa_tree_tc_splits(const TreeArgs& a);
+int sdpa_tree_tc(const TreeArgs& a, float* partials, cudaStream_t st);
+
 struct MassArgs {
   int dtype;
   uint32_t n, h, h_kv, l, s, e;
