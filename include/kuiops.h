@@ -374,6 +374,8 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
 /* A KV cache across decode steps: trees of drafted tokens, bounded size    */
 /* ======================================================================== */
 #define KUIOPS_TREE_MAX_ROWS 4096u
+/* Most entry points of this section take their arguments as one block: passing forty arguments through a foreign
+ * function interface costs more than the work of a small call.  A block is read before the call returns. */
 
 /* Attention of l drafted tokens (a tree, or any set of candidate continuations) over a cache plus their own
  * keys and values, which are not in the cache yet: row i of batch entry b sees the cache keys j < kv_lens[b]
@@ -390,17 +392,22 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
  * contents required; calls that may overlap on the GPU need workspaces of their own.  No counterpart in the reference. */
 KUIOPS_API size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
                                    uint32_t l, uint32_t s, uint32_t e, uint32_t ev);
-KUIOPS_API int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
-                uint32_t l, uint32_t s, uint32_t e, uint32_t ev,
-                const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
-                const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                const void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                const int64_t* kv_lens,
-                const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
-                const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
-                const void* mask, int64_t mask_sn, float scale,
-                void* out, int64_t o_sn, int64_t o_sh, int64_t o_sl, float* lse,
-                void* workspace, size_t workspace_bytes, kuiops_stream_t stream);
+typedef struct kuiops_sdpa_tree_args {
+  const void *Q, *K, *V, *DK, *DV;
+  const uint8_t* mask;
+  const int64_t* kv_lens;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t q_sn, q_sh, q_sl, k_sn, k_sh, k_ss, v_sn, v_sh, v_ss;
+  int64_t dk_sn, dk_sh, dk_sl, dv_sn, dv_sh, dv_sl, o_sn, o_sh, o_sl, mask_sn;
+  uint64_t workspace_bytes;
+  int32_t dtype;
+  uint32_t n, h, h_kv, l, s, e, ev;
+  float scale;
+  uint32_t reserved;
+} kuiops_sdpa_tree_args;
+KUIOPS_API int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream);
 
 /* Greedy acceptance of a verified tree.  parents is [l] int64 per sequence (parents_sn elements from one sequence to
  * the next, 0: one tree for all): parents[0] = -1 (the root is the token that is certain), parents[i] < i, and -1
@@ -421,14 +428,18 @@ KUIOPS_API int kuiops_tree_accept(uint32_t n, uint32_t l, const int64_t* parents
  * kv_lens[g] + counts[g], at most cap; kv_lens itself is not written, and the call may be repeated.  Elements of
  * 1, 2 or 4 bytes.  A row or slot out of range is skipped and stores 1 in *status (which may be NULL).  No counterpart
  * in the reference (its caches grow by cat, kuiops/cat/wrapper_cat.cu.j2:28-34). */
-KUIOPS_API int kuiops_kv_append(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t l, uint32_t cap, uint32_t e, uint32_t ev,
-                const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
-                const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
-                void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                const int64_t* kv_lens, uint32_t lens_n, const int64_t* path, const int64_t* counts,
-                int32_t* pos, const int64_t* next_pos, float* mass, int64_t* lens_out,
-                int32_t* status, kuiops_stream_t stream);
+typedef struct kuiops_kv_append_args {
+  const void *DK, *DV;
+  void *K, *V;
+  const int64_t *kv_lens, *path, *counts, *next_pos;
+  int32_t* pos;
+  float* mass;
+  int64_t* lens_out;
+  int32_t* status;
+  int64_t dk_sn, dk_sh, dk_sl, dv_sn, dv_sh, dv_sl, k_sn, k_sh, k_ss, v_sn, v_sh, v_ss;
+  uint32_t elem_bytes, n, h_kv, l, cap, e, ev, lens_n;
+} kuiops_kv_append_args;
+KUIOPS_API int kuiops_kv_append(const kuiops_kv_append_args* args, kuiops_stream_t stream);
 
 /* The attention weight each key has received: for every slot j < s of every KV head
  *     out[b, kh, j] = mass[b, kh, j] + sum over the query heads of kh and the rows i with j < lim_i of
@@ -439,11 +450,19 @@ KUIOPS_API int kuiops_kv_append(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, 
  * a row out.  mass == NULL counts as zeros; mass may be out.  Slots at or beyond kv_lens[g] keep their mass.
  * Q (n, h, l, e) and K (n, h_kv, s, e) as in kuiops_sdpa; mass and out are dense (n, h_kv, s) fp32.  fp32 accumulation in a
  * fixed order.  e <= 1024 (KUIOPS_EUNSUPPORTED beyond).  No counterpart in the reference. */
-KUIOPS_API int kuiops_attn_mass(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
-                const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
-                const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                const float* lse, const int64_t* kv_lens, uint32_t lens_n, const int64_t* q_lens,
-                float scale, int is_causal, const float* mass, float* out, kuiops_stream_t stream);
+typedef struct kuiops_attn_mass_args {
+  const void *Q, *K;
+  const float* lse;
+  const int64_t *kv_lens, *q_lens;
+  const float* mass;
+  float* out;
+  int64_t q_sn, q_sh, q_sl, k_sn, k_sh, k_ss;
+  int32_t dtype;
+  uint32_t n, h, h_kv, l, s, e, lens_n;
+  int32_t is_causal;
+  float scale;
+} kuiops_attn_mass_args;
+KUIOPS_API int kuiops_attn_mass(const kuiops_attn_mass_args* args, kuiops_stream_t stream);
 
 /* Keeps `budget` of the kv_lens[g] slots of every (batch, KV head) row of a cache (g = b % lens_n): first the protected
  * ones (0 <= pos < sinks, or pos >= next_pos[g] - recent), then those with the largest mass (NaN above +inf, as
@@ -458,13 +477,20 @@ KUIOPS_API int kuiops_attn_mass(int dtype, uint32_t n, uint32_t h, uint32_t h_kv
  * workspace: kuiops_kv_evict_workspace_bytes(...) bytes, 4-byte aligned, no initial contents required.  No counterpart
  * in the reference. */
 KUIOPS_API size_t kuiops_kv_evict_workspace_bytes(uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t budget);
-KUIOPS_API int kuiops_kv_evict(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t e, uint32_t ev,
-                void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                const float* mass, const int32_t* pos, const int64_t* kv_lens, const int64_t* next_pos, uint32_t lens_n,
-                uint32_t budget, uint32_t sinks, uint32_t recent,
-                float* mass_out, int32_t* pos_out, int32_t* src, int64_t* lens_out,
-                void* workspace, size_t workspace_bytes, kuiops_stream_t stream);
+typedef struct kuiops_kv_evict_args {
+  void *K, *V;
+  const float* mass;
+  const int32_t* pos;
+  const int64_t *kv_lens, *next_pos;
+  float* mass_out;
+  int32_t *pos_out, *src;
+  int64_t* lens_out;
+  void* workspace;
+  int64_t k_sn, k_sh, k_ss, v_sn, v_sh, v_ss;
+  uint64_t workspace_bytes;
+  uint32_t elem_bytes, n, h_kv, cap, e, ev, lens_n, budget, sinks, recent;
+} kuiops_kv_evict_args;
+KUIOPS_API int kuiops_kv_evict(const kuiops_kv_evict_args* args, kuiops_stream_t stream);
 
 /* ======================================================================== */
 /* Streaming reductions                                                     */

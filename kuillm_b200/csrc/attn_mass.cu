@@ -9,6 +9,8 @@
 
 namespace kuiops {
 
+static_assert(sizeof(kuiops_attn_mass_args) == 144, "callers pack the block without padding");
+
 constexpr float kMassLog2e = 1.4426950408889634f;
 constexpr int kMassRows = 16;                    // query rows staged at a time
 
@@ -113,24 +115,17 @@ using namespace kuiops;
 
 extern "C" {
 
-int kuiops_attn_mass(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
-                     const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
-                     const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                     const float* lse, const int64_t* kv_lens, uint32_t lens_n, const int64_t* q_lens,
-                     float scale, int is_causal, const float* mass, float* out, kuiops_stream_t stream) {
-  if (dtype != KUIOPS_F32 && dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_EINVAL;
-  if (n == 0 || h == 0 || h_kv == 0 || l == 0 || s == 0 || e == 0 || h % h_kv) return KUIOPS_EINVAL;
-  if (!Q || !K || !lse || !out || q_sl < int64_t(e) || k_ss < int64_t(e)) return KUIOPS_EINVAL;
-  if ((kv_lens || q_lens) && (lens_n == 0 || n % lens_n)) return KUIOPS_EINVAL;
-  if (!(scale - scale == 0.f)) return KUIOPS_EINVAL;
-  if (e > 1024) return KUIOPS_EUNSUPPORTED;
-  if (s > 0x7fffff00u || uint64_t(h / h_kv) * l >= (1ull << 31)) return KUIOPS_ELIMIT;
-  MassArgs a = {};
-  a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e;
-  a.Q = Q; a.q_sn = q_sn; a.q_sh = q_sh; a.q_sl = q_sl;
-  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
-  a.lse = lse; a.kv_lens = kv_lens; a.lens_n = lens_n ? lens_n : 1; a.q_lens = q_lens;
-  a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.mass = mass; a.out = out;
+int kuiops_attn_mass(const kuiops_attn_mass_args* args, kuiops_stream_t stream) {
+  if (!args) return KUIOPS_EINVAL;
+  MassArgs a = *args;
+  if (a.dtype != KUIOPS_F32 && a.dtype != KUIOPS_BF16 && a.dtype != KUIOPS_F16) return KUIOPS_EINVAL;
+  if (a.n == 0 || a.h == 0 || a.h_kv == 0 || a.l == 0 || a.s == 0 || a.e == 0 || a.h % a.h_kv) return KUIOPS_EINVAL;
+  if (!a.Q || !a.K || !a.lse || !a.out || a.q_sl < int64_t(a.e) || a.k_ss < int64_t(a.e)) return KUIOPS_EINVAL;
+  if ((a.kv_lens || a.q_lens) && (a.lens_n == 0 || a.n % a.lens_n)) return KUIOPS_EINVAL;
+  if (!(a.scale - a.scale == 0.f)) return KUIOPS_EINVAL;
+  if (a.e > 1024) return KUIOPS_EUNSUPPORTED;
+  if (a.s > 0x7fffff00u || uint64_t(a.h / a.h_kv) * a.l >= (1ull << 31)) return KUIOPS_ELIMIT;
+  if (a.lens_n == 0) a.lens_n = 1;
   return attn_mass_simt(a, as_stream(stream));
 }
 

@@ -4,6 +4,8 @@
 
 namespace kuiops {
 
+static_assert(sizeof(kuiops_kv_append_args) == 224, "callers pack the block without padding");
+
 constexpr int kAcceptThreads = 128;
 
 // One CTA per sequence.  Node i is accepted when every node j on its way to the root (itself included, the root not)
@@ -47,16 +49,7 @@ tree_accept_kernel(uint32_t l, const int64_t* __restrict__ parents, int64_t par_
   }
 }
 
-struct AppendArgs {
-  uint32_t elem_bytes, n, h_kv, l, cap, e, ev, lens_n;
-  const void* DK; int64_t dk_sn, dk_sh, dk_sl;
-  const void* DV; int64_t dv_sn, dv_sh, dv_sl;
-  void* K; int64_t k_sn, k_sh, k_ss;
-  void* V; int64_t v_sn, v_sh, v_ss;
-  const int64_t *kv_lens, *path, *counts, *next_pos;
-  int32_t* pos; float* mass; int64_t* lens_out; int32_t* status;
-  int wide;                             // every row of both tensors starts on a 16-byte boundary and is whole vectors
-};
+using AppendArgs = kuiops_kv_append_args;
 
 __device__ __forceinline__ void copy_row(const char* src, char* dst, uint32_t bytes, uint32_t elem, int wide, uint32_t lane) {
   if (wide) {
@@ -72,7 +65,7 @@ __device__ __forceinline__ void copy_row(const char* src, char* dst, uint32_t by
 
 // blockIdx.x: batch entry * parts + part.  A warp moves one accepted row of one KV head (K, then V) at a time.
 __global__ void __launch_bounds__(256)
-kv_append_kernel(const AppendArgs p, uint32_t parts) {
+kv_append_kernel(const AppendArgs p, uint32_t parts, int wide) {
   const uint32_t b = blockIdx.x / parts, part = blockIdx.x % parts, g = b % p.lens_n;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -95,9 +88,9 @@ kv_append_kernel(const AppendArgs p, uint32_t parts) {
     }
     const uint32_t eb = p.elem_bytes;
     copy_row(static_cast<const char*>(p.DK) + (int64_t(b) * p.dk_sn + int64_t(kvh) * p.dk_sh + row * p.dk_sl) * eb,
-             static_cast<char*>(p.K) + (int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh + slot * p.k_ss) * eb, p.e * eb, eb, p.wide, lane);
+             static_cast<char*>(p.K) + (int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh + slot * p.k_ss) * eb, p.e * eb, eb, wide, lane);
     copy_row(static_cast<const char*>(p.DV) + (int64_t(b) * p.dv_sn + int64_t(kvh) * p.dv_sh + row * p.dv_sl) * eb,
-             static_cast<char*>(p.V) + (int64_t(b) * p.v_sn + int64_t(kvh) * p.v_sh + slot * p.v_ss) * eb, p.ev * eb, eb, p.wide, lane);
+             static_cast<char*>(p.V) + (int64_t(b) * p.v_sn + int64_t(kvh) * p.v_sh + slot * p.v_ss) * eb, p.ev * eb, eb, wide, lane);
     if (lane == 0) {
       const size_t at = (size_t(b) * p.h_kv + kvh) * p.cap + size_t(slot);
       if (p.pos) p.pos[at] = int32_t(p.next_pos[g] + t);
@@ -121,37 +114,27 @@ int kuiops_tree_accept(uint32_t n, uint32_t l, const int64_t* parents, int64_t p
                     target, path, counts, next, status);
 }
 
-int kuiops_kv_append(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t l, uint32_t cap, uint32_t e, uint32_t ev,
-                     const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
-                     const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
-                     void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                     void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                     const int64_t* kv_lens, uint32_t lens_n, const int64_t* path, const int64_t* counts,
-                     int32_t* pos, const int64_t* next_pos, float* mass, int64_t* lens_out, int32_t* status, kuiops_stream_t stream) {
+int kuiops_kv_append(const kuiops_kv_append_args* args, kuiops_stream_t stream) {
+  if (!args) return KUIOPS_EINVAL;
+  const AppendArgs& a = *args;
+  const uint32_t elem_bytes = a.elem_bytes, n = a.n, h_kv = a.h_kv, l = a.l, e = a.e, ev = a.ev;
   if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return KUIOPS_EINVAL;
-  if (n == 0 || h_kv == 0 || l == 0 || cap == 0 || e == 0 || ev == 0 || lens_n == 0 || n % lens_n) return KUIOPS_EINVAL;
-  if (!DK || !DV || !K || !V || !kv_lens || (pos && !next_pos)) return KUIOPS_EINVAL;
-  if (dk_sl < int64_t(e) || dv_sl < int64_t(ev) || k_ss < int64_t(e) || v_ss < int64_t(ev)) return KUIOPS_EINVAL;
-  if (cap > 0x7fffff00u || uint64_t(l) * h_kv >= (1ull << 31) || uint64_t(e > ev ? e : ev) * 4 >= (1ull << 31)) return KUIOPS_ELIMIT;
-  AppendArgs a = {};
-  a.elem_bytes = elem_bytes; a.n = n; a.h_kv = h_kv; a.l = l; a.cap = cap; a.e = e; a.ev = ev; a.lens_n = lens_n;
-  a.DK = DK; a.dk_sn = dk_sn; a.dk_sh = dk_sh; a.dk_sl = dk_sl;
-  a.DV = DV; a.dv_sn = dv_sn; a.dv_sh = dv_sh; a.dv_sl = dv_sl;
-  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
-  a.V = V; a.v_sn = v_sn; a.v_sh = v_sh; a.v_ss = v_ss;
-  a.kv_lens = kv_lens; a.path = path; a.counts = counts; a.next_pos = next_pos;
-  a.pos = pos; a.mass = mass; a.lens_out = lens_out; a.status = status;
+  if (n == 0 || h_kv == 0 || l == 0 || a.cap == 0 || e == 0 || ev == 0 || a.lens_n == 0 || n % a.lens_n) return KUIOPS_EINVAL;
+  if (!a.DK || !a.DV || !a.K || !a.V || !a.kv_lens || (a.pos && !a.next_pos)) return KUIOPS_EINVAL;
+  if (a.dk_sl < int64_t(e) || a.dv_sl < int64_t(ev) || a.k_ss < int64_t(e) || a.v_ss < int64_t(ev)) return KUIOPS_EINVAL;
+  if (a.cap > 0x7fffff00u || uint64_t(l) * h_kv >= (1ull << 31) || uint64_t(e > ev ? e : ev) * 4 >= (1ull << 31)) return KUIOPS_ELIMIT;
   auto whole = [&](const void* t, uint32_t f, int64_t sn, int64_t sh, int64_t sl) {
     const int64_t v = 16 / elem_bytes;
     return aligned16(t) && f % v == 0 && (n == 1 || sn % v == 0) && (h_kv == 1 || sh % v == 0) && sl % v == 0;
   };
-  a.wide = whole(DK, e, dk_sn, dk_sh, dk_sl) && whole(DV, ev, dv_sn, dv_sh, dv_sl) && whole(K, e, k_sn, k_sh, k_ss) &&
-           whole(V, ev, v_sn, v_sh, v_ss);
+  // every row of all four tensors starts on a 16-byte boundary and is whole vectors
+  const int wide = whole(a.DK, e, a.dk_sn, a.dk_sh, a.dk_sl) && whole(a.DV, ev, a.dv_sn, a.dv_sh, a.dv_sl) &&
+                   whole(a.K, e, a.k_sn, a.k_sh, a.k_ss) && whole(a.V, ev, a.v_sn, a.v_sh, a.v_ss);
   // one CTA per 64 rows that could be accepted: those that are not cost a look at the count
   const uint64_t parts64 = (uint64_t(l) * h_kv + 63) / 64;
   const uint32_t parts = uint32_t(parts64 > 16 ? 16 : parts64);
   if (uint64_t(n) * parts >= (1ull << 31)) return KUIOPS_ELIMIT;
-  return launch_pdl(kv_append_kernel, dim3(n * parts), dim3(256), 0, as_stream(stream), a, parts);
+  return launch_pdl(kv_append_kernel, dim3(n * parts), dim3(256), 0, as_stream(stream), a, parts, wide);
 }
 
 }  // extern "C"

@@ -9,18 +9,15 @@
 
 namespace kuiops {
 
+static_assert(sizeof(kuiops_kv_evict_args) == 184, "callers pack the block without padding");
+
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWarps = kEvictThreads / 32;
 
-struct EvictArgs {
-  uint32_t elem_bytes, n, h_kv, cap, e, ev, budget, sinks, recent, lens_n;
-  void* K; int64_t k_sn, k_sh, k_ss;
-  void* V; int64_t v_sn, v_sh, v_ss;
-  const float* mass; const int32_t* pos; const int64_t *kv_lens, *next_pos;
-  float* mass_out; int32_t* pos_out; int32_t* src; int64_t* lens_out;
-  int32_t *holes, *movers, *moves;      // workspace: per row up to `pairs` (hole, mover) slots and their number
+struct EvictArgs : kuiops_kv_evict_args {
+  int32_t *holes, *movers, *moves;      // in the workspace: per row up to `pairs` (hole, mover) slots, and their number
   uint32_t pairs;
-  int wide;
+  int wide;                             // every row of K and V starts on a 16-byte boundary and is whole vectors
 };
 
 // Order-preserving image of a slot's weight: NaN above +inf, protected slots above all.
@@ -218,38 +215,30 @@ size_t kuiops_kv_evict_workspace_bytes(uint32_t n, uint32_t h_kv, uint32_t cap, 
   return size_t(n) * h_kv * 4 * (2 * size_t(evict_pairs(cap, budget)) + 1);
 }
 
-int kuiops_kv_evict(uint32_t elem_bytes, uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t e, uint32_t ev,
-                    void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                    void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                    const float* mass, const int32_t* pos, const int64_t* kv_lens, const int64_t* next_pos, uint32_t lens_n,
-                    uint32_t budget, uint32_t sinks, uint32_t recent,
-                    float* mass_out, int32_t* pos_out, int32_t* src, int64_t* lens_out,
-                    void* workspace, size_t workspace_bytes, kuiops_stream_t stream) {
-  if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return KUIOPS_EINVAL;
-  if (n == 0 || h_kv == 0 || cap == 0 || e == 0 || ev == 0 || budget == 0 || lens_n == 0 || n % lens_n) return KUIOPS_EINVAL;
-  if (!K || !V || !mass || !kv_lens || !mass_out || !pos_out || !src || !lens_out) return KUIOPS_EINVAL;
-  if (mass_out == mass || pos_out == pos || lens_out == kv_lens || k_ss < int64_t(e) || v_ss < int64_t(ev)) return KUIOPS_EINVAL;
-  if (budget > cap || uint64_t(sinks) + recent > budget) return KUIOPS_EINVAL;
-  if (cap > 0x7fffff00u || uint64_t(n) * h_kv >= (1ull << 31) || uint64_t(e > ev ? e : ev) * 4 >= (1ull << 31)) return KUIOPS_ELIMIT;
-  if (!workspace || workspace_bytes < kuiops_kv_evict_workspace_bytes(n, h_kv, cap, budget) || (reinterpret_cast<uintptr_t>(workspace) & 3))
-    return KUIOPS_EWORKSPACE;
+int kuiops_kv_evict(const kuiops_kv_evict_args* args, kuiops_stream_t stream) {
+  if (!args) return KUIOPS_EINVAL;
   EvictArgs a = {};
-  a.elem_bytes = elem_bytes; a.n = n; a.h_kv = h_kv; a.cap = cap; a.e = e; a.ev = ev;
-  a.budget = budget; a.sinks = sinks; a.recent = recent; a.lens_n = lens_n;
-  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
-  a.V = V; a.v_sn = v_sn; a.v_sh = v_sh; a.v_ss = v_ss;
-  a.mass = mass; a.pos = pos; a.kv_lens = kv_lens; a.next_pos = next_pos;
-  a.mass_out = mass_out; a.pos_out = pos_out; a.src = src; a.lens_out = lens_out;
+  static_cast<kuiops_kv_evict_args&>(a) = *args;
+  const uint32_t elem_bytes = a.elem_bytes, n = a.n, h_kv = a.h_kv, e = a.e, ev = a.ev;
+  if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return KUIOPS_EINVAL;
+  if (n == 0 || h_kv == 0 || a.cap == 0 || e == 0 || ev == 0 || a.budget == 0 || a.lens_n == 0 || n % a.lens_n) return KUIOPS_EINVAL;
+  if (!a.K || !a.V || !a.mass || !a.kv_lens || !a.mass_out || !a.pos_out || !a.src || !a.lens_out) return KUIOPS_EINVAL;
+  if (a.mass_out == a.mass || a.pos_out == a.pos || a.lens_out == a.kv_lens || a.k_ss < int64_t(e) || a.v_ss < int64_t(ev)) return KUIOPS_EINVAL;
+  if (a.budget > a.cap || uint64_t(a.sinks) + a.recent > a.budget) return KUIOPS_EINVAL;
+  if (a.cap > 0x7fffff00u || uint64_t(n) * h_kv >= (1ull << 31) || uint64_t(e > ev ? e : ev) * 4 >= (1ull << 31)) return KUIOPS_ELIMIT;
+  if (!a.workspace || a.workspace_bytes < kuiops_kv_evict_workspace_bytes(n, h_kv, a.cap, a.budget) ||
+      (reinterpret_cast<uintptr_t>(a.workspace) & 3))
+    return KUIOPS_EWORKSPACE;
   const uint32_t rows = n * h_kv;
-  a.pairs = evict_pairs(cap, budget);
-  a.moves = static_cast<int32_t*>(workspace);
+  a.pairs = evict_pairs(a.cap, a.budget);
+  a.moves = static_cast<int32_t*>(a.workspace);
   a.holes = a.moves + rows;
   a.movers = a.holes + size_t(rows) * a.pairs;
   auto whole = [&](const void* t, uint32_t f, int64_t sn, int64_t sh, int64_t sl) {
     const int64_t v = 16 / elem_bytes;
     return aligned16(t) && f % v == 0 && (n == 1 || sn % v == 0) && (h_kv == 1 || sh % v == 0) && sl % v == 0;
   };
-  a.wide = whole(K, e, k_sn, k_sh, k_ss) && whole(V, ev, v_sn, v_sh, v_ss);
+  a.wide = whole(a.K, e, a.k_sn, a.k_sh, a.k_ss) && whole(a.V, ev, a.v_sn, a.v_sh, a.v_ss);
   cudaStream_t st = as_stream(stream);
   const int rc = launch_pdl(kv_evict_select_kernel, dim3(rows), dim3(kEvictThreads), 0, st, a);
   if (rc != KUIOPS_OK || a.pairs == 0) return rc;

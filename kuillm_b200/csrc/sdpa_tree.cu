@@ -9,6 +9,8 @@
 
 namespace kuiops {
 
+static_assert(sizeof(kuiops_sdpa_tree_args) == 280, "callers pack the block without padding");
+
 constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeLn2 = 0.6931471805599453f;
 
@@ -50,7 +52,7 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
   const T* Vb = static_cast<const T*>(p.V) + int64_t(b) * p.v_sn + int64_t(kvh) * p.v_sh;
   const T* Kd = static_cast<const T*>(p.DK) + int64_t(b) * p.dk_sn + int64_t(kvh) * p.dk_sh;
   const T* Vd = static_cast<const T*>(p.DV) + int64_t(b) * p.dv_sn + int64_t(kvh) * p.dv_sh;
-  const unsigned char* mk = p.mask + int64_t(b) * p.m_sn;
+  const unsigned char* mk = p.mask + int64_t(b) * p.mask_sn;
 
   float m[R], lsum[R], acc[R][DV];
 #pragma unroll
@@ -262,12 +264,11 @@ int sdpa_tree_merge(const TreeArgs& a, const float* partials, uint32_t splits, c
 
 using namespace kuiops;
 
-static int tree_shape(TreeArgs& a, int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev) {
+static int tree_shape(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev) {
   if (dtype != KUIOPS_F32 && dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_EINVAL;
   if (n == 0 || h == 0 || h_kv == 0 || l == 0 || e == 0 || ev == 0 || h % h_kv) return KUIOPS_EINVAL;
   if (e > 1024 || ev > 256) return KUIOPS_EUNSUPPORTED;
   if (l > KUIOPS_TREE_MAX_ROWS || s > 0x7fffff00u || uint64_t(n) * h * l >= (1ull << 31)) return KUIOPS_ELIMIT;
-  a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e; a.ev = ev;
   return KUIOPS_OK;
 }
 
@@ -280,44 +281,30 @@ extern "C" {
 size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
                                         uint32_t ev) {
   TreeArgs a = {};
-  if (tree_shape(a, dtype, n, h, h_kv, l, s, e, ev) != KUIOPS_OK) return 0;
+  if (tree_shape(dtype, n, h, h_kv, l, s, e, ev) != KUIOPS_OK) return 0;
+  a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e; a.ev = ev;
   // which kernel runs also depends on alignment, unknown here: cover both
   const uint32_t simt = sdpa_tree_simt_splits(a);
   const uint32_t tc = dtype != KUIOPS_F32 && e <= 128 && ev <= 128 && h / h_kv <= 128 ? sdpa_tree_tc_splits(a) : 1;
   return tree_record_bytes(a, simt > tc ? simt : tc);
 }
 
-int kuiops_sdpa_tree(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev,
-                     const void* Q, int64_t q_sn, int64_t q_sh, int64_t q_sl,
-                     const void* K, int64_t k_sn, int64_t k_sh, int64_t k_ss,
-                     const void* V, int64_t v_sn, int64_t v_sh, int64_t v_ss,
-                     const int64_t* kv_lens,
-                     const void* DK, int64_t dk_sn, int64_t dk_sh, int64_t dk_sl,
-                     const void* DV, int64_t dv_sn, int64_t dv_sh, int64_t dv_sl,
-                     const void* mask, int64_t mask_sn, float scale,
-                     void* out, int64_t o_sn, int64_t o_sh, int64_t o_sl, float* lse,
-                     void* workspace, size_t workspace_bytes, kuiops_stream_t stream) {
-  TreeArgs a = {};
-  const int rc = tree_shape(a, dtype, n, h, h_kv, l, s, e, ev);
+int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream) {
+  if (!args) return KUIOPS_EINVAL;
+  const TreeArgs& a = *args;
+  const int rc = tree_shape(a.dtype, a.n, a.h, a.h_kv, a.l, a.s, a.e, a.ev);
   if (rc != KUIOPS_OK) return rc;
-  if (!Q || !DK || !DV || !mask || !out || (s > 0 && (!K || !V))) return KUIOPS_EINVAL;
-  if (q_sl < int64_t(e) || dk_sl < int64_t(e) || dv_sl < int64_t(ev) || o_sl < int64_t(ev)) return KUIOPS_EINVAL;
-  if (s > 0 && (k_ss < int64_t(e) || v_ss < int64_t(ev))) return KUIOPS_EINVAL;
-  if (mask_sn != 0 && mask_sn < int64_t(l) * l) return KUIOPS_EINVAL;
-  if (!(scale - scale == 0.f)) return KUIOPS_EINVAL;              // a finite number
-  a.Q = Q; a.q_sn = q_sn; a.q_sh = q_sh; a.q_sl = q_sl;
-  a.K = K; a.k_sn = k_sn; a.k_sh = k_sh; a.k_ss = k_ss;
-  a.V = V; a.v_sn = v_sn; a.v_sh = v_sh; a.v_ss = v_ss;
-  a.kv_lens = kv_lens;
-  a.DK = DK; a.dk_sn = dk_sn; a.dk_sh = dk_sh; a.dk_sl = dk_sl;
-  a.DV = DV; a.dv_sn = dv_sn; a.dv_sh = dv_sh; a.dv_sl = dv_sl;
-  a.mask = static_cast<const unsigned char*>(mask); a.m_sn = mask_sn;
-  a.scale = scale; a.out = out; a.o_sn = o_sn; a.o_sh = o_sh; a.o_sl = o_sl; a.lse = lse;
+  if (!a.Q || !a.DK || !a.DV || !a.mask || !a.out || (a.s > 0 && (!a.K || !a.V))) return KUIOPS_EINVAL;
+  const int64_t e = a.e, ev = a.ev;
+  if (a.q_sl < e || a.dk_sl < e || a.dv_sl < ev || a.o_sl < ev) return KUIOPS_EINVAL;
+  if (a.s > 0 && (a.k_ss < e || a.v_ss < ev)) return KUIOPS_EINVAL;
+  if (a.mask_sn != 0 && a.mask_sn < int64_t(a.l) * a.l) return KUIOPS_EINVAL;
+  if (!(a.scale - a.scale == 0.f)) return KUIOPS_EINVAL;          // a finite number
   cudaStream_t st = as_stream(stream);
   const bool tc = sdpa_tree_tc_eligible(a);
   const uint32_t splits = tc ? sdpa_tree_tc_splits(a) : sdpa_tree_simt_splits(a);
-  if (splits > 1 && (!workspace || workspace_bytes < tree_record_bytes(a, splits) || !aligned16(workspace))) return KUIOPS_EWORKSPACE;
-  float* partials = static_cast<float*>(workspace);
+  if (splits > 1 && (!a.workspace || a.workspace_bytes < tree_record_bytes(a, splits) || !aligned16(a.workspace))) return KUIOPS_EWORKSPACE;
+  float* partials = static_cast<float*>(a.workspace);
   const int run = tc ? sdpa_tree_tc(a, partials, st) : sdpa_tree_simt(a, partials, splits, st);
   if (run != KUIOPS_OK || splits == 1) return run;
   return sdpa_tree_merge(a, partials, splits, st);

@@ -230,7 +230,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const bool row_valid = r < p.rows && li < a.l;
     const uint32_t lane_addr = (quarter * 32) << 16;
     const uint32_t tid = threadIdx.x - 64;
-    const unsigned char* mrow = a.mask + int64_t(b) * a.m_sn + size_t(row_valid ? li : 0) * a.l;
+    const unsigned char* mrow = a.mask + int64_t(b) * a.mask_sn + size_t(row_valid ? li : 0) * a.l;
     float m_used = -INFINITY, l_run = 0.f;
     bool ok = true;
     for (uint32_t j = 0; j < n_tiles && ok; ++j) {
@@ -402,7 +402,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
         if (odd) {
           // drafted elements that were taken out of the product, for the rows that see them
-          const unsigned char* mr = a.mask + int64_t(b) * a.m_sn + size_t(pos) * a.l;
+          const unsigned char* mr = a.mask + int64_t(b) * a.mask_sn + size_t(pos) * a.l;
           const uint32_t d_lo = t_lo > cache_tiles ? (t_lo - cache_tiles) * RTN : 0;
           const uint32_t d_hi = t_hi > cache_tiles ? min((t_hi - cache_tiles) * RTN, a.l) : 0;
           for (uint32_t k = d_lo; k < d_hi; ++k) {

@@ -9,6 +9,7 @@ raises.
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -92,16 +93,12 @@ SIGNATURES = {
                             [c_void_p, c_i64, c_i64, c_i64] * 3 +
                             [c_void_p, c_float, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_void_p]),
     "kuiops_sdpa_tree_workspace_bytes": (c_size_t, [c_int] + [c_u32] * 7),
-    "kuiops_sdpa_tree": (c_int, [c_int] + [c_u32] * 7 + [c_void_p, c_i64, c_i64, c_i64] * 3 + [c_void_p] +
-                         [c_void_p, c_i64, c_i64, c_i64] * 2 + [c_void_p, c_i64, c_float] +
-                         [c_void_p, c_i64, c_i64, c_i64] + [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "kuiops_sdpa_tree": (c_int, [c_void_p, c_void_p]),
     "kuiops_tree_accept": (c_int, [c_u32, c_u32, c_void_p, c_i64] + [c_void_p] * 7),
-    "kuiops_kv_append": (c_int, [c_u32] * 7 + [c_void_p, c_i64, c_i64, c_i64] * 4 + [c_void_p, c_u32] + [c_void_p] * 8),
-    "kuiops_attn_mass": (c_int, [c_int] + [c_u32] * 6 + [c_void_p, c_i64, c_i64, c_i64] * 2 +
-                         [c_void_p, c_void_p, c_u32, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p]),
+    "kuiops_kv_append": (c_int, [c_void_p, c_void_p]),
+    "kuiops_attn_mass": (c_int, [c_void_p, c_void_p]),
     "kuiops_kv_evict_workspace_bytes": (c_size_t, [c_u32] * 4),
-    "kuiops_kv_evict": (c_int, [c_u32] * 6 + [c_void_p, c_i64, c_i64, c_i64] * 2 + [c_void_p] * 4 + [c_u32] * 4 +
-                        [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "kuiops_kv_evict": (c_int, [c_void_p, c_void_p]),
     "kuiops_add_i64": (c_int, [c_u64, c_void_p, c_i64, c_void_p]),
     "kuiops_topk_f32": (c_int, [c_u32, c_u32, c_u32, c_void_p, c_void_p, c_void_p, c_void_p]),
     "kuiops_gather": (c_int, [c_u32, c_u32, c_u32, _P64, _P64, c_void_p, c_void_p, c_void_p, c_u64,
@@ -552,43 +549,51 @@ def sdpa(Q, K, V, *, bias=None, scale=None, is_causal=False, need_lse=True, out=
 # --------------------------------------------------------------------------------------------
 # a KV cache across decode steps: trees of drafted tokens, bounded size
 # --------------------------------------------------------------------------------------------
-def _require(ok, what):
-    if not ok:
-        raise KuiopsError(EINVAL, what)
+# the argument blocks of include/kuiops.h, field for field: pointers and strides, then counts
+_TREE_ARGS = struct.Struct("=30Qi7IfI")
+_APPEND_ARGS = struct.Struct("=24Q8I")
+_MASS_ARGS = struct.Struct("=13Qi7Iif")
+_EVICT_ARGS = struct.Struct("=18Q10I")
 
 
-def _on_device(dev, what, *tensors):
-    """Every tensor on the CUDA device `dev`; returns a context that makes it the current one (None: it is)."""
+def _refuse(what):
+    raise KuiopsError(EINVAL, what)
+
+
+def _elsewhere(dev, what, *tensors):
+    """Refuses tensors that are not all on the CUDA device number `dev`; a context that makes it current if it is not."""
+    if dev < 0:
+        _refuse(f"{what}: needs CUDA tensors")
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise KuiopsError(EINVAL, f"{what}: tensors on {t.device} and {dev}")
-    if dev.type != "cuda":
-        raise KuiopsError(EINVAL, f"{what}: needs CUDA tensors, got {dev}")
-    return None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            _refuse(f"{what}: tensors on different devices")
+    return None if dev == (_cur_device() if _cur_device is not None else torch.cuda.current_device()) else torch.cuda.device(dev)
 
 
 def _rows_last(t):
-    """Strides of a 4-D tensor whose innermost dimension is contiguous (a copy of it otherwise)."""
-    st = t.stride()
-    if st[3] != 1 and t.shape[3] != 1 or st[2] < t.shape[3]:
+    """Strides of a 4-D tensor whose innermost dimension is contiguous and whose rows do not overlap (a copy of it otherwise)."""
+    a, b, c, d = t.stride()
+    e = t.shape[3]
+    if d != 1 or c < e or a < 0 or b < 0:
         t = t.contiguous()
-        st = t.stride()
-        if st[2] < t.shape[3]:                  # a single row may carry any stride
-            st = (st[0], st[1], t.shape[3], 1)
-    return t, st
+        a, b, c, d = t.stride()
+        if c < e:                               # a single row may carry any stride
+            c = e
+    return t, a, b, c
 
 
 def _own_rows(t):
     """A 4-D tensor that rows can be written to one by one: contiguous innermost, no two rows the same memory."""
     n, hkv, rows, e = t.shape
     a, b, c, d = t.stride()
-    return (e == 1 or d == 1) and (rows == 1 or c >= e) and (hkv == 1 or b > 0) and (n == 1 or a > 0)
+    return (e == 1 or d == 1) and (rows == 1 or c >= e) and (hkv == 1 or b >= e) and (n == 1 or a >= e)
 
 
 def _dense(t, dtype, what):
     if t is None:
         return None
-    _require(t.dtype == dtype, f"{what} has to be {dtype}")
+    if t.dtype is not dtype:
+        _refuse(f"{what} has to be {dtype}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -596,44 +601,49 @@ def sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, *, scale=None, need_lse=True, out=
     """Attention of drafted tokens over a cache: Q (n,h,l,e), cache K / V (n,h_kv,s,e|ev) with kv_lens [n] int64 keys
     in use (None: all s), the drafted tokens' own keys and values Kd / Vd (n,h_kv,l,e|ev), mask bool [l,l] or
     [n,l,l] (row i sees drafted key j) -> out (n,h,l,ev), lse (n,h,l) fp32 or None."""
-    _require(Q.dim() == 4 and K.dim() == 4 and V.dim() == 4 and Kd.dim() == 4 and Vd.dim() == 4, "sdpa_tree: 4-D tensors")
+    if not (Q.dim() == 4 and K.dim() == 4 and V.dim() == 4):
+        _refuse("sdpa_tree: 4-D tensors")
     n, h, l, e = Q.shape
-    _, hkv, s, _ = K.shape
-    ev = V.shape[3]
-    _require(K.shape == (n, hkv, s, e) and V.shape == (n, hkv, s, ev) and Kd.shape == (n, hkv, l, e) and Vd.shape == (n, hkv, l, ev),
-             "sdpa_tree: shapes of Q, the cache and the drafted rows")
+    hkv, s, ev = K.shape[1], K.shape[2], V.shape[3]
+    if not (K.shape == (n, hkv, s, e) and V.shape == (n, hkv, s, ev) and Kd.shape == (n, hkv, l, e) and Vd.shape == (n, hkv, l, ev)):
+        _refuse("sdpa_tree: shapes of Q, the cache and the drafted rows")
     dt = Q.dtype
-    _require(K.dtype == dt and V.dtype == dt and Kd.dtype == dt and Vd.dtype == dt, "sdpa_tree: one element type")
-    _require(mask.dtype in (torch.bool, torch.uint8) and mask.shape in ((l, l), (1, l, l), (n, l, l)), "sdpa_tree: mask [l,l] or [n,l,l] of bool")
+    if not (K.dtype is dt and V.dtype is dt and Kd.dtype is dt and Vd.dtype is dt):
+        _refuse("sdpa_tree: one element type")
+    if not (mask.dtype is torch.bool or mask.dtype is torch.uint8) or mask.shape not in ((n, l, l), (l, l), (1, l, l)):
+        _refuse("sdpa_tree: mask [l,l] or [n,l,l] of bool")
     kv_lens = _dense(kv_lens, torch.int64, "sdpa_tree: kv_lens")
-    _require(kv_lens is None or kv_lens.numel() == n, "sdpa_tree: one key count per batch entry")
-    _require(out is None or (out.shape == (n, h, l, ev) and out.dtype == dt and (out.stride(3) == 1 or ev == 1)), "sdpa_tree: out")
-    dev = Q.device
-    ctx = _on_device(dev, "sdpa_tree", K, V, kv_lens, Kd, Vd, mask, out)
+    if kv_lens is not None and kv_lens.numel() != n:
+        _refuse("sdpa_tree: one key count per batch entry")
+    if out is not None and not (out.shape == (n, h, l, ev) and out.dtype is dt and _own_rows(out)):
+        _refuse("sdpa_tree: out")
+    dev = Q.get_device()
+    ctx = _elsewhere(dev, "sdpa_tree", K, V, kv_lens, Kd, Vd, mask, out)
     if ctx is not None:
         with ctx:
             return sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, scale=scale, need_lse=need_lse, out=out)
-    Q, qs = _rows_last(Q)
-    K, ks = _rows_last(K)
-    V, vs = _rows_last(V)
-    Kd, ds = _rows_last(Kd)
-    Vd, es = _rows_last(Vd)
+    Q, q0, q1, q2 = _rows_last(Q)
+    K, k0, k1, k2 = _rows_last(K)
+    V, v0, v1, v2 = _rows_last(V)
+    Kd, d0, d1, d2 = _rows_last(Kd)
+    Vd, e0, e1, e2 = _rows_last(Vd)
     if not mask.is_contiguous():
         mask = mask.contiguous()
     if out is None:
-        out = torch.empty((n, h, l, ev), dtype=dt, device=dev)
-    os_ = out.stride()
-    lse = torch.empty((n, h, l), dtype=torch.float32, device=dev) if need_lse else None
+        out = Q.new_empty((n, h, l, ev))
+    o0, o1, o2, _ = out.stride()
+    lse = torch.empty((n, h, l), dtype=torch.float32, device=out.device) if need_lse else None
     L = lib()
     code = dtype_code(dt)
     wsb = L.kuiops_sdpa_tree_workspace_bytes(code, n, h, hkv, l, s, e, ev)
     # a buffer of this call alone: captured graphs keep theirs, and calls on several streams do not meet
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-    _check(L.kuiops_sdpa_tree(code, n, h, hkv, l, s, e, ev, Q.data_ptr(), qs[0], qs[1], qs[2], K.data_ptr(), ks[0], ks[1], ks[2],
-                              V.data_ptr(), vs[0], vs[1], vs[2], _ptr(kv_lens), Kd.data_ptr(), ds[0], ds[1], ds[2],
-                              Vd.data_ptr(), es[0], es[1], es[2], mask.data_ptr(), l * l if mask.dim() == 3 and mask.shape[0] > 1 else 0,
-                              1.0 / (e ** 0.5) if scale is None else float(scale), out.data_ptr(), os_[0], os_[1], max(os_[2], ev),
-                              _ptr(lse), _ptr(ws), wsb, _stream()), "sdpa_tree")
+    ws = torch.empty(wsb, dtype=torch.uint8, device=out.device) if wsb else None
+    _check(L.kuiops_sdpa_tree(_TREE_ARGS.pack(
+        Q.data_ptr(), K.data_ptr(), V.data_ptr(), Kd.data_ptr(), Vd.data_ptr(), mask.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr(),
+        q0, q1, q2, k0, k1, k2, v0, v1, v2, d0, d1, d2, e0, e1, e2, o0, o1, o2 if o2 > ev else ev,
+        l * l if mask.dim() == 3 and mask.shape[0] > 1 else 0, wsb,
+        code, n, h, hkv, l, s, e, ev, e ** -0.5 if scale is None else scale, 0), _stream()), "sdpa_tree")
     return out, lse
 
 
@@ -641,20 +651,21 @@ def tree_accept(parents, draft, target):
     """Greedy walk through a verified tree: parents [l] or [n,l], draft and target [n,l] (int64) -> path [n,l] (the
     accepted nodes from the root, then -1), counts [n], next token [n].  parents[0] = -1 is the root, parents[i] < i,
     -1 elsewhere marks padding."""
-    _require(draft.dim() == 2 and target.shape == draft.shape, "tree_accept: draft and target [n,l]")
+    if draft.dim() != 2 or target.shape != draft.shape:
+        _refuse("tree_accept: draft and target [n,l]")
     n, l = draft.shape
-    _require(parents.shape in ((l,), (1, l), (n, l)), "tree_accept: parents [l] or [n,l]")
+    if parents.shape not in ((l,), (1, l), (n, l)):
+        _refuse("tree_accept: parents [l] or [n,l]")
     parents, draft, target = (_dense(t, torch.int64, "tree_accept: tokens and parents") for t in (parents, draft, target))
-    dev = draft.device
-    ctx = _on_device(dev, "tree_accept", parents, target)
+    dev = draft.get_device()
+    ctx = _elsewhere(dev, "tree_accept", parents, target)
     if ctx is not None:
         with ctx:
             return tree_accept(parents, draft, target)
-    path = torch.empty((n, l), dtype=torch.int64, device=dev)
-    both = torch.empty((2, n), dtype=torch.int64, device=dev)
-    counts, nxt = both[0], both[1]
+    path = torch.empty_like(draft)
+    counts, nxt = draft.new_empty((2, n)).unbind(0)
     _check(lib().kuiops_tree_accept(n, l, parents.data_ptr(), l if parents.dim() == 2 and parents.shape[0] > 1 else 0, draft.data_ptr(),
-                                    target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status(dev).data_ptr(),
+                                    target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status(draft.device).data_ptr(),
                                     _stream()), "tree_accept")
     return path, counts, nxt
 
@@ -664,33 +675,43 @@ def kv_append(K, V, kv_lens, Kn, Vn, *, path=None, counts=None, pos=None, next_p
     to slot kv_lens[g] + t for t < counts[g] (all l without counts).  kv_lens [g] int64 with n a multiple of g: entry b
     uses b % g, so the layers of a model go in one call.  pos int32 and mass fp32 (n,h_kv,cap) are set for the new slots
     (next_pos[g] + t and 0).  Returns the new key counts [g]."""
-    _require(K.dim() == 4 and V.dim() == 4 and Kn.dim() == 4 and Vn.dim() == 4, "kv_append: 4-D tensors")
+    if not (K.dim() == 4 and V.dim() == 4 and Kn.dim() == 4):
+        _refuse("kv_append: 4-D tensors")
     n, hkv, cap, e = K.shape
     l, ev = Kn.shape[2], V.shape[3]
-    _require(V.shape == (n, hkv, cap, ev) and Kn.shape == (n, hkv, l, e) and Vn.shape == (n, hkv, l, ev), "kv_append: shapes of caches and rows")
-    _require(V.dtype == K.dtype and Kn.dtype == K.dtype and Vn.dtype == K.dtype, "kv_append: one element type")
-    _require(_own_rows(K) and _own_rows(V), "kv_append: cache rows have to be contiguous, and rows of their own")
-    kv_lens, path, counts, next_pos = (_dense(t, torch.int64, "kv_append: counts, positions and path") for t in (kv_lens, path, counts, next_pos))
+    if not (V.shape == (n, hkv, cap, ev) and Kn.shape == (n, hkv, l, e) and Vn.shape == (n, hkv, l, ev)):
+        _refuse("kv_append: shapes of caches and rows")
+    dt = K.dtype
+    if not (V.dtype is dt and Kn.dtype is dt and Vn.dtype is dt):
+        _refuse("kv_append: one element type")
+    if not (_own_rows(K) and _own_rows(V)):
+        _refuse("kv_append: cache rows have to be contiguous, and rows of their own")
+    what = "kv_append: counts, positions and path"
+    kv_lens, path, counts, next_pos = _dense(kv_lens, torch.int64, what), _dense(path, torch.int64, what), _dense(counts, torch.int64, what), _dense(next_pos, torch.int64, what)
     g = kv_lens.numel()
-    _require(g > 0 and n % g == 0 and (path is None or path.shape == (g, l)) and (counts is None or counts.numel() == g)
-             and (next_pos is None or next_pos.numel() == g), "kv_append: one entry of kv_lens, path, counts and next_pos per sequence")
-    _require(pos is None or (next_pos is not None and pos.dtype == torch.int32 and pos.shape == (n, hkv, cap) and pos.is_contiguous()),
-             "kv_append: pos is a dense int32 (n, h_kv, cap) and needs next_pos")
-    _require(mass is None or (mass.dtype == torch.float32 and mass.shape == (n, hkv, cap) and mass.is_contiguous()),
-             "kv_append: mass is a dense fp32 (n, h_kv, cap)")
-    dev = K.device
-    ctx = _on_device(dev, "kv_append", V, kv_lens, Kn, Vn, path, counts, pos, next_pos, mass)
+    if g == 0 or n % g or (path is not None and path.shape != (g, l)) or (counts is not None and counts.numel() != g) \
+            or (next_pos is not None and next_pos.numel() != g):
+        _refuse("kv_append: one entry of kv_lens, path, counts and next_pos per sequence")
+    if pos is not None and not (next_pos is not None and pos.dtype is torch.int32 and pos.shape == (n, hkv, cap) and pos.is_contiguous()):
+        _refuse("kv_append: pos is a dense int32 (n, h_kv, cap) and needs next_pos")
+    if mass is not None and not (mass.dtype is torch.float32 and mass.shape == (n, hkv, cap) and mass.is_contiguous()):
+        _refuse("kv_append: mass is a dense fp32 (n, h_kv, cap)")
+    dev = K.get_device()
+    ctx = _elsewhere(dev, "kv_append", V, kv_lens, Kn, Vn, path, counts, pos, next_pos, mass)
     if ctx is not None:
         with ctx:
             return kv_append(K, V, kv_lens, Kn, Vn, path=path, counts=counts, pos=pos, next_pos=next_pos, mass=mass)
-    Kn, ds = _rows_last(Kn)
-    Vn, es = _rows_last(Vn)
-    ks, vs = K.stride(), V.stride()
-    lens_out = torch.empty(g, dtype=torch.int64, device=dev)
-    _check(lib().kuiops_kv_append(K.element_size(), n, hkv, l, cap, e, ev, Kn.data_ptr(), ds[0], ds[1], ds[2], Vn.data_ptr(), es[0], es[1], es[2],
-                                  K.data_ptr(), ks[0], ks[1], max(ks[2], e), V.data_ptr(), vs[0], vs[1], max(vs[2], ev), kv_lens.data_ptr(), g,
-                                  _ptr(path), _ptr(counts), _ptr(pos), _ptr(next_pos), _ptr(mass), lens_out.data_ptr(),
-                                  _status(dev).data_ptr(), _stream()), "kv_append")
+    Kn, d0, d1, d2 = _rows_last(Kn)
+    Vn, e0, e1, e2 = _rows_last(Vn)
+    k0, k1, k2, _ = K.stride()
+    v0, v1, v2, _ = V.stride()
+    lens_out = torch.empty_like(kv_lens)
+    _check(lib().kuiops_kv_append(_APPEND_ARGS.pack(
+        Kn.data_ptr(), Vn.data_ptr(), K.data_ptr(), V.data_ptr(), kv_lens.data_ptr(), 0 if path is None else path.data_ptr(),
+        0 if counts is None else counts.data_ptr(), 0 if next_pos is None else next_pos.data_ptr(), 0 if pos is None else pos.data_ptr(),
+        0 if mass is None else mass.data_ptr(), lens_out.data_ptr(), _status(K.device).data_ptr(),
+        d0, d1, d2, e0, e1, e2, k0, k1, k2 if k2 > e else e, v0, v1, v2 if v2 > ev else ev,
+        K.element_size(), n, hkv, l, cap, e, ev, g), _stream()), "kv_append")
     return lens_out
 
 
@@ -699,30 +720,34 @@ def attn_mass(Q, K, lse, *, kv_lens=None, q_lens=None, is_causal=True, scale=Non
     whose log-sum-exp lse (n,h,l) an attention call returned.  kv_lens [g] (n a multiple of g): keys in use; row i counts for
     its first q_lens[g,i] keys, or (is_causal) i + 1 + kv_lens - l, or all.  A row whose lse is infinite is left out.  out
     may be mass."""
-    _require(Q.dim() == 4 and K.dim() == 4, "attn_mass: 4-D tensors")
+    if not (Q.dim() == 4 and K.dim() == 4):
+        _refuse("attn_mass: 4-D tensors")
     n, h, l, e = Q.shape
-    _, hkv, s, _ = K.shape
-    _require(K.shape == (n, hkv, s, e) and K.dtype == Q.dtype, "attn_mass: shapes and type of Q and K")
-    _require(lse.shape == (n, h, l), "attn_mass: lse (n,h,l)")
-    lse = _dense(lse, torch.float32, "attn_mass: lse")
+    hkv, s = K.shape[1], K.shape[2]
+    if K.shape != (n, hkv, s, e) or K.dtype is not Q.dtype or lse.shape != (n, h, l):
+        _refuse("attn_mass: shapes and type of Q, K and lse")
+    lse, mass = _dense(lse, torch.float32, "attn_mass: lse"), _dense(mass, torch.float32, "attn_mass: mass")
     kv_lens, q_lens = _dense(kv_lens, torch.int64, "attn_mass: kv_lens"), _dense(q_lens, torch.int64, "attn_mass: q_lens")
     g = kv_lens.numel() if kv_lens is not None else (q_lens.shape[0] if q_lens is not None else 1)
-    _require(g > 0 and n % g == 0 and (q_lens is None or q_lens.shape == (g, l)), "attn_mass: one key count per sequence")
-    _require(mass is None or mass.shape == (n, hkv, s), "attn_mass: mass (n,h_kv,s)")
-    mass = _dense(mass, torch.float32, "attn_mass: mass")
-    _require(out is None or (out.shape == (n, hkv, s) and out.dtype == torch.float32 and out.is_contiguous()), "attn_mass: out is a dense fp32 (n,h_kv,s)")
-    dev = Q.device
-    ctx = _on_device(dev, "attn_mass", K, lse, kv_lens, q_lens, mass, out)
+    if g == 0 or n % g or (q_lens is not None and q_lens.shape != (g, l)):
+        _refuse("attn_mass: one key count per sequence")
+    if mass is not None and mass.shape != (n, hkv, s):
+        _refuse("attn_mass: mass (n,h_kv,s)")
+    if out is not None and not (out.shape == (n, hkv, s) and out.dtype is torch.float32 and out.is_contiguous()):
+        _refuse("attn_mass: out is a dense fp32 (n,h_kv,s)")
+    dev = Q.get_device()
+    ctx = _elsewhere(dev, "attn_mass", K, lse, kv_lens, q_lens, mass, out)
     if ctx is not None:
         with ctx:
             return attn_mass(Q, K, lse, kv_lens=kv_lens, q_lens=q_lens, is_causal=is_causal, scale=scale, mass=mass, out=out)
-    Q, qs = _rows_last(Q)
-    K, ks = _rows_last(K)
+    Q, q0, q1, q2 = _rows_last(Q)
+    K, k0, k1, k2 = _rows_last(K)
     if out is None:
-        out = torch.empty((n, hkv, s), dtype=torch.float32, device=dev)
-    _check(lib().kuiops_attn_mass(dtype_code(Q.dtype), n, h, hkv, l, s, e, Q.data_ptr(), qs[0], qs[1], qs[2], K.data_ptr(), ks[0], ks[1], ks[2],
-                                  lse.data_ptr(), _ptr(kv_lens), g, _ptr(q_lens), 1.0 / (e ** 0.5) if scale is None else float(scale),
-                                  1 if is_causal else 0, _ptr(mass), out.data_ptr(), _stream()), "attn_mass")
+        out = lse.new_empty((n, hkv, s))
+    _check(lib().kuiops_attn_mass(_MASS_ARGS.pack(
+        Q.data_ptr(), K.data_ptr(), lse.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(),
+        0 if mass is None else mass.data_ptr(), out.data_ptr(), q0, q1, q2, k0, k1, k2,
+        dtype_code(Q.dtype), n, h, hkv, l, s, e, g, 1 if is_causal else 0, e ** -0.5 if scale is None else scale), _stream()), "attn_mass")
     return out
 
 
@@ -731,34 +756,42 @@ def kv_evict(K, V, mass, kv_lens, budget, *, pos=None, next_pos=None, sinks=0, r
     `sinks`, or among the last `recent` before next_pos), then those with the largest mass (n,h_kv,cap).  kv_lens [g] int64
     with n a multiple of g.  K and V rows move in place; returns (new key counts [g], mass, positions, src) with src
     (n,h_kv,budget) the slot each slot came from.  The inputs mass, pos and kv_lens stay as they are."""
-    _require(K.dim() == 4 and V.dim() == 4, "kv_evict: 4-D caches")
+    if not (K.dim() == 4 and V.dim() == 4):
+        _refuse("kv_evict: 4-D caches")
     n, hkv, cap, e = K.shape
     ev = V.shape[3]
-    _require(V.shape == (n, hkv, cap, ev) and V.dtype == K.dtype, "kv_evict: shapes and type of the caches")
-    _require(_own_rows(K) and _own_rows(V), "kv_evict: cache rows have to be contiguous, and rows of their own")
-    _require(mass.shape == (n, hkv, cap) and (pos is None or pos.shape == (n, hkv, cap)), "kv_evict: mass and pos (n,h_kv,cap)")
+    if V.shape != (n, hkv, cap, ev) or V.dtype is not K.dtype:
+        _refuse("kv_evict: shapes and type of the caches")
+    if not (_own_rows(K) and _own_rows(V)):
+        _refuse("kv_evict: cache rows have to be contiguous, and rows of their own")
+    if mass.shape != (n, hkv, cap) or (pos is not None and pos.shape != (n, hkv, cap)):
+        _refuse("kv_evict: mass and pos (n,h_kv,cap)")
     mass, pos = _dense(mass, torch.float32, "kv_evict: mass"), _dense(pos, torch.int32, "kv_evict: pos")
     kv_lens, next_pos = _dense(kv_lens, torch.int64, "kv_evict: kv_lens"), _dense(next_pos, torch.int64, "kv_evict: next_pos")
     g = kv_lens.numel()
-    budget, sinks, recent = int(budget), int(sinks), int(recent)
-    _require(g > 0 and n % g == 0 and (next_pos is None or next_pos.numel() == g), "kv_evict: one key count per sequence")
-    _require(1 <= budget <= cap and sinks >= 0 and recent >= 0 and sinks + recent <= budget, "kv_evict: 1 <= budget <= cap, sinks + recent <= budget")
-    dev = K.device
-    ctx = _on_device(dev, "kv_evict", V, mass, kv_lens, pos, next_pos)
+    if g == 0 or n % g or (next_pos is not None and next_pos.numel() != g):
+        _refuse("kv_evict: one key count per sequence")
+    if not (1 <= budget <= cap and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
+        _refuse("kv_evict: 1 <= budget <= cap, sinks + recent <= budget")
+    dev = K.get_device()
+    ctx = _elsewhere(dev, "kv_evict", V, mass, kv_lens, pos, next_pos)
     if ctx is not None:
         with ctx:
             return kv_evict(K, V, mass, kv_lens, budget, pos=pos, next_pos=next_pos, sinks=sinks, recent=recent)
-    mass_out = torch.empty((n, hkv, cap), dtype=torch.float32, device=dev)
-    pos_out = torch.empty((n, hkv, cap), dtype=torch.int32, device=dev)
-    src = torch.empty((n, hkv, budget), dtype=torch.int32, device=dev)
-    lens_out = torch.empty(g, dtype=torch.int64, device=dev)
+    mass_out = torch.empty_like(mass)
+    pos_out = torch.empty((n, hkv, cap), dtype=torch.int32, device=mass.device) if pos is None else torch.empty_like(pos)
+    src = pos_out.new_empty((n, hkv, budget))
+    lens_out = torch.empty_like(kv_lens)
     L = lib()
     wsb = L.kuiops_kv_evict_workspace_bytes(n, hkv, cap, budget)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    ks, vs = K.stride(), V.stride()
-    _check(L.kuiops_kv_evict(K.element_size(), n, hkv, cap, e, ev, K.data_ptr(), ks[0], ks[1], max(ks[2], e), V.data_ptr(), vs[0], vs[1], max(vs[2], ev),
-                             mass.data_ptr(), _ptr(pos), kv_lens.data_ptr(), _ptr(next_pos), g, budget, sinks, recent, mass_out.data_ptr(),
-                             pos_out.data_ptr(), src.data_ptr(), lens_out.data_ptr(), ws.data_ptr(), wsb, _stream()), "kv_evict")
+    ws = pos_out.new_empty((wsb + 3) // 4)
+    k0, k1, k2, _ = K.stride()
+    v0, v1, v2, _ = V.stride()
+    _check(L.kuiops_kv_evict(_EVICT_ARGS.pack(
+        K.data_ptr(), V.data_ptr(), mass.data_ptr(), 0 if pos is None else pos.data_ptr(), kv_lens.data_ptr(),
+        0 if next_pos is None else next_pos.data_ptr(), mass_out.data_ptr(), pos_out.data_ptr(), src.data_ptr(), lens_out.data_ptr(), ws.data_ptr(),
+        k0, k1, k2 if k2 > e else e, v0, v1, v2 if v2 > ev else ev, wsb,
+        K.element_size(), n, hkv, cap, e, ev, g, budget, sinks, recent), _stream()), "kv_evict")
     return lens_out, mass_out, pos_out, src
 
 

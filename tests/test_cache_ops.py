@@ -6,7 +6,9 @@ a score is a sum of e products, off by at most ds = (e + 8) 2^-24 scale sum|q k|
 off by a factor of at most 1 +- (2 ds + 2^-20 + keys 2^-24) (score and maximum, the exponential and the scaling to the
 log2 domain of values below 32, the sum), and 16-bit types round each weight once more (u) before the product with
 V; the result is rounded once (u)."""
-import ctypes
+import re
+import struct
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -17,6 +19,7 @@ from oracle import kuiops_oracle as O
 
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 U = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 0.0}
+HEADER = (Path(__file__).resolve().parent.parent / "include" / "kuiops.h").read_text()
 P = 0x1000                               # a non-null pointer that is never dereferenced
 
 
@@ -91,39 +94,58 @@ def test_append_accept_mass_evict_refusals_of_the_binding():
         assert refused(_ffi.kv_evict, *a, **kw) == _ffi.EINVAL
 
 
+def block(name):
+    """Field names of an argument block of the header, in order, and a packer that takes them by name (0 unless given)."""
+    body = re.search(r"typedef struct kuiops_%s_args \{(.*?)\}" % name, HEADER, re.S).group(1)
+    fields = []
+    for decl in body.split(";")[:-1]:
+        kind = "q" if "*" in decl or "int64_t" in decl else ("f" if "float" in decl else "i" if re.search(r"\bint32_t", decl) else "I")
+        names = re.sub(r"\b(const|void|float|u?int\d+_t)\b|\*", " ", decl)
+        fields += [(x.strip(), "Q" if kind == "q" and "uint64" not in decl else kind.upper() if "uint64" in decl else kind) for x in names.split(",")]
+    packer = getattr(_ffi, {"sdpa_tree": "_TREE_ARGS", "kv_append": "_APPEND_ARGS", "attn_mass": "_MASS_ARGS", "kv_evict": "_EVICT_ARGS"}[name])
+    fmt = packer.format if isinstance(packer.format, str) else packer.format.decode()
+    assert struct.Struct("=" + "".join(k for _, k in fields)).size == packer.size == struct.calcsize("@" + fmt[1:])
+    return [f for f, _ in fields], packer
+
+
+def c_call(name, defaults):
+    fields, packer = block(name)
+    fn = getattr(_ffi.lib(), "kuiops_" + name)
+
+    def call(**kw):
+        a = {**defaults, **kw}
+        assert set(a) <= set(fields), set(a) - set(fields)
+        return fn(packer.pack(*[a.get(f, 0) for f in fields]), None)
+    return call
+
+
 def test_contracts_of_the_c_entries():
     L = _ffi.lib()
-
-    def tree(dtype=_ffi.BF16, n=1, h=4, hkv=2, l=3, s=10, e=128, ev=128, q=P, k=P, ksl=128, mask=P, msn=0, scale=0.1, ws=P, wsb=1 << 30):
-        return L.kuiops_sdpa_tree(dtype, n, h, hkv, l, s, e, ev, q, 0, 0, e, k, 0, 0, ksl, P, 0, 0, ev, None, P, 0, 0, e, P, 0, 0, ev,
-                                  mask, msn, scale, P, 0, 0, ev, None, ws, wsb, None)
-    assert tree(dtype=7) == tree(n=0) == tree(l=0) == tree(h=3) == tree(q=None) == tree(k=None) == tree(mask=None) == _ffi.EINVAL
-    assert tree(ksl=64) == tree(msn=8) == tree(scale=float("nan")) == tree(scale=float("inf")) == _ffi.EINVAL
+    for name in ("sdpa_tree", "kv_append", "attn_mass", "kv_evict"):
+        assert getattr(L, "kuiops_" + name)(None, None) == _ffi.EINVAL
+    tree = c_call("sdpa_tree", dict(dtype=_ffi.BF16, n=1, h=4, h_kv=2, l=3, s=10, e=128, ev=128, Q=P, K=P, V=P, DK=P, DV=P, mask=P, out=P, workspace=P,
+                                    workspace_bytes=1 << 30, q_sl=128, k_ss=128, v_ss=128, dk_sl=128, dv_sl=128, o_sl=128, scale=0.1))
+    assert tree(dtype=7) == tree(n=0) == tree(l=0) == tree(h=3) == tree(Q=0) == tree(K=0) == tree(mask=0) == tree(out=0) == _ffi.EINVAL
+    assert tree(k_ss=64) == tree(mask_sn=8) == tree(scale=float("nan")) == tree(scale=float("inf")) == _ffi.EINVAL
     assert tree(e=2048) == tree(ev=512) == _ffi.EUNSUPPORTED and tree(l=5000) == _ffi.ELIMIT
     need = L.kuiops_sdpa_tree_workspace_bytes(_ffi.BF16, 1, 4, 2, 3, 100000, 128, 128)
     assert need > 0
-    assert tree(s=100000, ws=None) == tree(s=100000, wsb=need - 1) == tree(s=100000, ws=P + 4) == _ffi.EWORKSPACE
+    assert tree(s=100000, workspace=0) == tree(s=100000, workspace_bytes=16) == tree(s=100000, workspace=P + 4) == _ffi.EWORKSPACE
     acc = lambda n=2, l=5, par=P, sn=0: L.kuiops_tree_accept(n, l, par, sn, P, P, P, P, P, None, None)        # noqa: E731
     assert acc(n=0) == acc(l=0) == acc(par=None) == acc(sn=4) == _ffi.EINVAL and acc(l=5000) == _ffi.ELIMIT
-
-    def app(eb=2, n=4, cap=8, lens=P, g=2, pos=None, nxt=None, ksl=128):
-        return L.kuiops_kv_append(eb, n, 2, 3, cap, 128, 128, P, 0, 0, 128, P, 0, 0, 128, P, 0, 0, ksl, P, 0, 0, 128, lens, g, None, None,
-                                  pos, nxt, None, None, None, None)
-    assert app(eb=8) == app(n=0) == app(cap=0) == app(lens=None) == app(g=3) == app(g=0) == app(pos=P) == app(ksl=64) == _ffi.EINVAL
+    app = c_call("kv_append", dict(elem_bytes=2, n=4, h_kv=2, l=3, cap=8, e=128, ev=128, lens_n=2, DK=P, DV=P, K=P, V=P, kv_lens=P,
+                                   dk_sl=128, dv_sl=128, k_ss=128, v_ss=128))
+    assert app(elem_bytes=8) == app(n=0) == app(cap=0) == app(kv_lens=0) == app(lens_n=3) == app(lens_n=0) == app(pos=P) == app(k_ss=64) == _ffi.EINVAL
     assert app(cap=0x7fffffff) == _ffi.ELIMIT
-
-    def mass(dtype=_ffi.BF16, s=8, q=P, lse=P, lens=None, g=1, e=128, scale=0.1):
-        return L.kuiops_attn_mass(dtype, 4, 4, 2, 3, s, e, q, 0, 0, e, P, 0, 0, e, lse, lens, g, None, scale, 1, None, P, None)
-    assert mass(dtype=9) == mass(s=0) == mass(q=None) == mass(lse=None) == mass(lens=P, g=3) == mass(scale=float("nan")) == _ffi.EINVAL
-    assert mass(e=2000) == _ffi.EUNSUPPORTED
-
-    def evict(eb=2, cap=100, budget=10, sinks=0, recent=0, g=2, mass=P, mass_out=P + 64, ws=P, wsb=1 << 30):
-        return L.kuiops_kv_evict(eb, 4, 2, cap, 128, 128, P, 0, 0, 128, P, 0, 0, 128, mass, None, P, None, g, budget, sinks, recent,
-                                 mass_out, P, P, P + 8, ws, wsb, None)
-    assert evict(eb=3) == evict(budget=0) == evict(budget=101) == evict(sinks=6, recent=5) == evict(g=3) == _ffi.EINVAL
-    assert evict(sinks=0xFFFFFFFF, recent=2) == evict(mass=None) == evict(mass_out=P) == _ffi.EINVAL
-    assert evict(ws=None) == evict(wsb=L.kuiops_kv_evict_workspace_bytes(4, 2, 100, 10) - 1) == evict(ws=P + 2) == _ffi.EWORKSPACE
-    assert ctypes.c_size_t(L.kuiops_kv_evict_workspace_bytes(4, 2, 100, 100)).value == 32
+    mass = c_call("attn_mass", dict(dtype=_ffi.BF16, n=4, h=4, h_kv=2, l=3, s=8, e=128, lens_n=1, Q=P, K=P, lse=P, out=P, q_sl=128, k_ss=128, scale=0.1))
+    assert mass(dtype=9) == mass(s=0) == mass(Q=0) == mass(lse=0) == mass(kv_lens=P, lens_n=3) == mass(scale=float("nan")) == _ffi.EINVAL
+    assert mass(e=2000, q_sl=2000, k_ss=2000) == _ffi.EUNSUPPORTED
+    evict = c_call("kv_evict", dict(elem_bytes=2, n=4, h_kv=2, cap=100, e=128, ev=128, lens_n=2, budget=10, K=P, V=P, mass=P, mass_out=P + 64, pos_out=P,
+                                    src=P, kv_lens=P, lens_out=P + 8, workspace=P, workspace_bytes=1 << 30, k_ss=128, v_ss=128))
+    assert evict(elem_bytes=3) == evict(budget=0) == evict(budget=101) == evict(sinks=6, recent=5) == evict(lens_n=3) == _ffi.EINVAL
+    assert evict(sinks=0xFFFFFFFF, recent=2) == evict(mass=0) == evict(mass_out=P) == evict(lens_out=P) == _ffi.EINVAL
+    short = L.kuiops_kv_evict_workspace_bytes(4, 2, 100, 10) - 1
+    assert evict(workspace=0) == evict(workspace_bytes=short) == evict(workspace=P + 2) == _ffi.EWORKSPACE
 
 
 # ------------------------------------------------------------------------------------------------
