@@ -126,7 +126,7 @@ int kuiops_attn_mass(const kuiops_attn_mass_args* args, kuiops_stream_t stream) 
   if (a.e > 1024) return KUIOPS_EUNSUPPORTED;
   if (a.s > 0x7fffff00u || uint64_t(a.h / a.h_kv) * a.l >= (1ull << 31)) return KUIOPS_ELIMIT;
   if (a.lens_n == 0) a.lens_n = 1;
-  return attn_mass_simt(a, as_stream(stream));
+  return attn_mass_tc_eligible(a) ? attn_mass_tc(a, as_stream(stream)) : attn_mass_simt(a, as_stream(stream));
 }
 
 }  // extern "C"

@@ -28,6 +28,8 @@ uint32_t sdpa_tree_tc_splits(const TreeArgs& a);
 int sdpa_tree_tc(const TreeArgs& a, float* partials, cudaStream_t st);
 
 int attn_mass_simt(const MassArgs& a, cudaStream_t st);
+bool attn_mass_tc_eligible(const MassArgs& a);
+int attn_mass_tc(const MassArgs& a, cudaStream_t st);
 
 __device__ __forceinline__ uint32_t clamp_len(long long v, uint32_t s) {
   return v < 0 ? 0u : (v < (long long)s ? uint32_t(v) : s);
