@@ -14,7 +14,11 @@
 
 namespace kuiops {
 
-constexpr int kMassThreads = 192;          // warp 0: TMA, warp 1: UMMA issue, warps 2-5: one key per thread
+// warp 0: TMA, warp 1: UMMA issue, then one group of four warps per 32 columns (one key per thread): two groups give the
+// wide tiles' exponentials four warps per scheduler to hide latencies with (one group of 64 columns: 588 us for the 8192-token
+// prompt, two: see below)
+template <int NQ> constexpr int kMassGroups = NQ == 64 ? 2 : 1;
+template <int NQ> constexpr int kMassThreads = 64 + 128 * kMassGroups<NQ>;
 constexpr uint32_t MKT = 128;              // keys per item
 constexpr uint32_t MQR = 64;               // query rows per tile, at most
 constexpr uint32_t kMassLens = 256;        // key counts kept in shared memory
@@ -26,7 +30,7 @@ template <int DD> struct MassTile {
   static constexpr uint32_t kKRing = DD == 128 ? 2 : 4;
   static constexpr uint32_t kQRing = DD == 128 ? 2 : 4;
   static constexpr uint32_t kBars = 1 + 2 * (kKRing + kQRing) + 8;
-  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + 16 + kMassLens * 4 + 2 * MQR * 8 + 16;
+  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + 16 + kMassLens * 4 + 8 * 64 * 8 + 2 * 128 * 4;
   static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 constexpr uint32_t kMassS = 4;             // score buffers of 64 columns
@@ -49,12 +53,15 @@ __device__ __forceinline__ bool mass_wait(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
-// The 128 weight threads meet; true for all of them when one has given up.
-__device__ __forceinline__ bool mass_meet(bool failed) {
-  uint32_t any;
-  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbar.red.or.pred p, 1, 128, q;\nselp.u32 %0, 1, 0, p;\n}"
-               : "=r"(any) : "r"(failed ? 1u : 0u) : "memory");
-  return any != 0;
+// (a0, a1) = (a0, a1) * s + (c0, c1) and (a0, a1) += (b0, b1) as packed instructions
+__device__ __forceinline__ void mass_fma2(float& a0, float& a1, float s, float c0, float c1) {
+  asm("{.reg .b64 ra, rb, rc;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %2};\n mov.b64 rc, {%3, %4};\n"
+      " fma.rn.f32x2 ra, ra, rb, rc;\n mov.b64 {%0, %1}, ra;}"
+      : "+f"(a0), "+f"(a1) : "f"(s), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mass_add2(float& a0, float& a1, float b0, float b1) {
+  asm("{.reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;}"
+      : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
 }
 
 // One (batch, KV head, key tile) and the row tiles that can see it.
@@ -81,10 +88,11 @@ __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t*
 }
 
 template <typename T, int DD, int NQ>
-__global__ void __launch_bounds__(kMassThreads, 2)
+__global__ void __launch_bounds__(kMassThreads<NQ>, 2)
 attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const MassTcParams p) {
   using MT = MassTile<DD>;
   constexpr uint32_t KR = MT::kKRing, QR = MT::kQRing;
+  constexpr int GROUPS = kMassGroups<NQ>, THREADS = kMassThreads<NQ>;
   extern __shared__ __align__(1024) unsigned char smem[];
   if ((tc::smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicCAS(p.err, 0u, 50u);
@@ -101,17 +109,15 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* s_empty = s_full + kMassS;   // kMassS
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + kMassS);
   uint32_t* lens_s = tmem_slot + 4;
-  float* row_lse = reinterpret_cast<float*>(lens_s + kMassLens);          // [2][MQR], log2 domain
-  uint32_t* row_lim = reinterpret_cast<uint32_t*>(row_lse + 2 * MQR);     // [2][MQR] keys the row counts for
-  uint32_t* low_lim = row_lim + 2 * MQR;                                  // [2][2] smallest limit of 32 rows
-
+  float* row_s = reinterpret_cast<float*>(lens_s + kMassLens);            // per warp [2][32] -lse (log2 domain) and [2][32] limits
+  float* part_s = row_s + 8 * 128;                                         // [2][128] sums of the second group
   const MassArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tc::prefetch_tmap(&tmQ); tc::prefetch_tmap(&tmK);
     for (uint32_t i = 0; i < KR; ++i) { tc::mbar_init(&k_full[i], 1); tc::mbar_init(&k_empty[i], 1); }
     for (uint32_t i = 0; i < QR; ++i) { tc::mbar_init(&q_full[i], 1); tc::mbar_init(&q_empty[i], 1); }
-    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], 4); }
+    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], 4 * GROUPS); }
     tc::fence_barrier_init();
   }
   if (warp == 1) {
@@ -121,7 +127,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (p.rows < NQ) {
     // rows of the tile that TMA does not fill feed columns nobody reads, but no stale bit patterns either
     const uint32_t per = (NQ - p.rows) * 8;
-    for (uint32_t i = threadIdx.x; i < per * QR * MT::kHalves; i += kMassThreads) {
+    for (uint32_t i = threadIdx.x; i < per * QR * MT::kHalves; i += THREADS) {
       const uint32_t blk = i / per, o = i % per;         // blk = stage * halves + half
       *reinterpret_cast<int4*>(q_s + blk * (MQR * 128) + p.rows * 128 + o * 16) = make_int4(0, 0, 0, 0);
     }
@@ -129,7 +135,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   }
   pdl_wait();
   if (a.kv_lens)
-    for (uint32_t i = threadIdx.x; i < min(a.lens_n, kMassLens); i += kMassThreads) lens_s[i] = clamp_len(a.kv_lens[i], a.s);
+    for (uint32_t i = threadIdx.x; i < min(a.lens_n, kMassLens); i += THREADS) lens_s[i] = clamp_len(a.kv_lens[i], a.s);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -197,81 +203,77 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
   } else {
     // ------------------------------ weights: one key per thread ---------------------------
-    const uint32_t quarter = warp & 3, key = quarter * 32 + lane, tid = threadIdx.x - 64;
-    const uint32_t lane_addr = (quarter * 32) << 16;
-    uint32_t nq = 0;
-    bool ok = true, gone = false;
-    for (uint32_t round = 0; !gone && mass_item(p, lens_s, round, it); ++round) {
+    const uint32_t quarter = warp & 3, key = quarter * 32 + lane, group = uint32_t(warp - 2) >> 2;
+    constexpr int W = NQ < 32 ? NQ : 32;                  // columns of this warp: group * 32 ..
+    const uint32_t s_base = tmem_base + ((quarter * 32) << 16) + group * 32;
+    float* nl_s = row_s + (warp - 2) * 128;
+    uint32_t* lim_s = reinterpret_cast<uint32_t*>(nl_s + 64);
+    const uint32_t row = group * 32 + lane, gh = row / p.lt, ri = row % p.lt;      // the row this lane looks after
+    const bool row_in = row < p.rows;
+    uint32_t nq = 0, n_item = 0;
+    bool ok = true;
+    for (uint32_t round = 0; mass_item(p, lens_s, round, it); ++round) {
       const uint32_t j = it.key0 + key;
       float total = 0.f;
-      // lse and limit of the row this thread looks after (threads 0 .. 63), one tile ahead
-      float ls = 0.f;
+      // -lse and limit of the lane's row, one tile ahead
+      float nl = 0.f;
       uint32_t lim = 0;
+      const float* lse_row = a.lse + (size_t(it.b) * a.h + it.kvh * p.G + gh) * a.l;
       auto fetch = [&](uint32_t qt) {
-        lim = 0; ls = 0.f;
-        if (tid < MQR && qt < it.qt1) {
-          const uint32_t li = qt * p.lt + tid % p.lt, gh = tid / p.lt;
-          if (tid < p.rows && li < a.l) {
-            ls = a.lse[(size_t(it.b) * a.h + it.kvh * p.G + gh) * a.l + li] * 1.4426950408889634f;
-            if (a.q_lens) lim = clamp_len(a.q_lens[size_t(it.g) * a.l + li], it.len);
-            else if (a.is_causal) lim = clamp_len((long long)li + 1 + (long long)it.len - (long long)a.l, it.len);
-            else lim = it.len;
-            if (isinf(ls)) { lim = 0; ls = 0.f; }     // saw nothing, or is not to be counted
-          }
+        const uint32_t li = qt * p.lt + ri;
+        nl = 0.f; lim = 0;
+        if (row_in && qt < it.qt1 && li < a.l) {
+          nl = -1.4426950408889634f * lse_row[li];
+          if (a.q_lens) lim = clamp_len(a.q_lens[size_t(it.g) * a.l + li], it.len);
+          else if (a.is_causal) lim = clamp_len((long long)li + 1 + (long long)it.len - (long long)a.l, it.len);
+          else lim = it.len;
         }
       };
       fetch(it.qt0);
       for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
-        const uint32_t buf = nq & 1, sb = nq % kMassS;
-        if (tid < MQR) {
-          row_lse[buf * MQR + tid] = -ls;
-          row_lim[buf * MQR + tid] = lim;
-          const uint32_t low = __reduce_min_sync(0xffffffffu, lim);
-          if (lane == 0) low_lim[buf * 2 + (tid >> 5)] = low;
-        }
+        const uint32_t buf = (nq & 1) * 32, sb = nq % kMassS;
+        if (isinf(nl)) { nl = 0.f; lim = 0; }             // saw nothing, or is not to be counted
+        nl_s[buf + lane] = nl;
+        lim_s[buf + lane] = lim;
+        const bool all = __all_sync(0xffffffffu, lim >= it.key0 + MKT);      // every row counts for every key of the tile
         fetch(qt + 1);
-        // two buffers and one meeting per tile: a thread that is a tile ahead writes the other buffer
-        gone = mass_meet(!ok);
-        if (gone) { ok = false; break; }
-        if (!__all_sync(0xffffffffu, mass_wait(&s_full[sb], (nq / kMassS) & 1))) { atomicCAS(p.err, 0u, 56u); ok = false; }
+        if (ok && !__all_sync(0xffffffffu, mass_wait(&s_full[sb], (nq / kMassS) & 1))) { atomicCAS(p.err, 0u, 56u); ok = false; }
         tc::tc_fence_after();
-        float sv[NQ];
-        if constexpr (NQ == 16) {
-          tc::tmem_ld16(tmem_base + sb * MQR + lane_addr, sv);
-        } else {
-          tc::tmem_ld32(tmem_base + sb * MQR + lane_addr, sv);
-          if constexpr (NQ == 64) tc::tmem_ld32(tmem_base + sb * MQR + lane_addr + 32, sv + 32);
-        }
+        float sv[W];
+        if constexpr (W == 16) tc::tmem_ld16(s_base + sb * MQR, sv);
+        else tc::tmem_ld32(s_base + sb * MQR, sv);
         tc::tmem_ld_wait();
         tc::tc_fence_before();
-        __syncwarp();
+        __syncwarp();                                      // the row's values are in place, too
         if (lane == 0) tc::mbar_arrive(&s_empty[sb]);
-        float r0 = 0.f, r1 = 0.f;
+        float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
+        if (all) {
 #pragma unroll
-        for (int c0 = 0; c0 < NQ; c0 += 32) {
-          constexpr int W = NQ < 32 ? NQ : 32;
-          const float* nl = row_lse + buf * MQR + c0;
-          if (low_lim[buf * 2 + c0 / 32] >= it.key0 + MKT) {      // every row counts for every key of the tile
+          for (int c = 0; c < W; c += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(nl_s + buf + c);
+            mass_fma2(sv[c], sv[c + 1], p.scale_log2, x.x, x.y);
+            mass_fma2(sv[c + 2], sv[c + 3], p.scale_log2, x.z, x.w);
+            mass_add2(r0, r1, fast_ex2(sv[c]), fast_ex2(sv[c + 1]));
+            mass_add2(r2, r3, fast_ex2(sv[c + 2]), fast_ex2(sv[c + 3]));
+          }
+        } else {
 #pragma unroll
-            for (int c = 0; c < W; c += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(nl + c);
-              float s0 = fmaf(sv[c0 + c], p.scale_log2, x.x), s1 = fmaf(sv[c0 + c + 1], p.scale_log2, x.y);
-              float s2 = fmaf(sv[c0 + c + 2], p.scale_log2, x.z), s3 = fmaf(sv[c0 + c + 3], p.scale_log2, x.w);
-              r0 += fast_ex2(s0) + fast_ex2(s1);
-              r1 += fast_ex2(s2) + fast_ex2(s3);
-            }
-          } else {
-            const uint32_t* lm = row_lim + buf * MQR + c0;
-#pragma unroll
-            for (int c = 0; c < W; ++c) {
-              const float w = fast_ex2(fmaf(sv[c0 + c], p.scale_log2, nl[c]));
-              r0 += j < lm[c] ? w : 0.f;
-            }
+          for (int c = 0; c < W; ++c) {
+            const float w = fast_ex2(fmaf(sv[c], p.scale_log2, nl_s[buf + c]));
+            r0 += j < lim_s[buf + c] ? w : 0.f;
           }
         }
-        total += r0 + r1;
+        total += (r0 + r1) + (r2 + r3);
       }
-      if (j < a.s) {
+      if constexpr (GROUPS == 2) {
+        // the second group's sums come through shared memory; two buffers and one meeting per item: a thread that is an item
+        // ahead writes the other buffer
+        float* part = part_s + (n_item++ & 1) * 128;
+        if (group == 1) part[key] = total;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (group == 0) total += part[key];
+      }
+      if (group == 0 && j < a.s) {
         const size_t o = (size_t(it.b) * a.h_kv + it.kvh) * a.s + j;
         if (a.mass != a.out || j < it.len) a.out[o] = (a.mass ? a.mass[o] : 0.f) + (j < it.len ? total : 0.f);
       }
@@ -309,7 +311,7 @@ static int mass_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const Ma
     configured.fetch_or(bit, std::memory_order_release);
   }
   const uint64_t items = uint64_t(p.units) * p.key_tiles, slots = 2ull * num_sms();
-  return launch_pdl(kern, dim3(unsigned(items < slots ? items : slots)), dim3(kMassThreads), smem, st, mq, mk, p);
+  return launch_pdl(kern, dim3(unsigned(items < slots ? items : slots)), dim3(kMassThreads<NQ>), smem, st, mq, mk, p);
 }
 
 template <typename T, int DD>
