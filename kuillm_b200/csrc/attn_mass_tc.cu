@@ -1,43 +1,50 @@
 // Attention weight received per key, on tcgen05 (16-bit types, up to 128 features per head).
 //
 // Scores are computed transposed, S^T = K Q^T: the 128 lanes of the tile are keys and the columns are query rows (G heads x
-// lt positions, at most 64).  A key's weight is then a sum along one thread's own columns - no exchange between threads, no
-// maximum (the rows' log-sum-exp is given), no second product - and what the thread holds at the end is the answer.
+// lt positions).  A key's weight is then a sum along one thread's own columns - no exchange between threads, no maximum (the
+// rows' log-sum-exp is given), no second product - and what the thread holds at the end is the answer.
 //
-// For a few rows the kernel is bound by reading K once from HBM: persistent CTAs, two to an SM, walk (batch, KV head,
-// 128-key tile) items and keep two K tiles in flight each.  For many rows it is bound by the exponentials (16 per clock and SM): the
-// rows' tiles stream past a resident K tile, four score buffers in TMEM keep the products ahead.  Items are dealt in
-// alternating direction, which evens out a causal mask's falling work per tile.
+// One persistent CTA per SM walks (batch, KV head, 128-key tile) items; four groups of four warps (a thread per key) make the
+// weights.
+//   Up to 64 rows per KV head (decode, a small window): bound by reading K once from HBM.  Four to eight K tiles are in flight,
+//   an item is one product, and the groups take items in turn, each with a score buffer of its own, so that a group's
+//   latencies (log-sum-exp, scores, the old mass) hide behind three other items.
+//   More rows (a window, a prompt): bound by the exponentials, 16 per clock and SM, then by the products.  Tiles of 128 rows
+//   stream past a resident K tile (128 columns: a 64-column product would be bound by shared memory, whose A operand it reads
+//   twice as often) and every group takes 32 columns of each.  A quarter of the exponentials is made by a polynomial in the FMA
+//   pipe instead of the special-function unit.  Items are dealt in alternating direction, which evens out a causal
+//   mask's falling work per item.
 #include "tree.cuh"
 #include "tc_ptx.cuh"
 #include <type_traits>
 
 namespace kuiops {
 
-// warp 0: TMA, warp 1: UMMA issue, then one group of four warps per 32 columns (one key per thread): two groups give the
-// wide tiles' exponentials four warps per scheduler to hide latencies with (one group of 64 columns: 588 us for the 8192-token
-// prompt, two: see below)
-template <int NQ> constexpr int kMassGroups = NQ == 64 ? 2 : 1;
-template <int NQ> constexpr int kMassThreads = 64 + 128 * kMassGroups<NQ>;
+constexpr int kMassGroups = 4;
+// warp 0: TMA, warp 1: UMMA issue, warps 2-17: weights, then a warp per 32 columns that prepares the rows' values
+template <int NQ> constexpr int kMassRowWarps = NQ < 32 ? 1 : NQ / 32;
+template <int NQ> constexpr int kMassThreads = 64 + 128 * kMassGroups + 32 * kMassRowWarps<NQ>;
 constexpr uint32_t MKT = 128;              // keys per item
-constexpr uint32_t MQR = 64;               // query rows per tile, at most
 constexpr uint32_t kMassLens = 256;        // key counts kept in shared memory
+constexpr uint32_t kMassS = 4;             // score buffers
 
-template <int DD> struct MassTile {
+// NQ columns per tile; 128 = the form that streams row tiles, else all rows are one tile.
+template <int DD, int NQ> struct MassTile {
+  static constexpr bool kStream = NQ == 128;
   static constexpr uint32_t kHalves = DD / 64;
   static constexpr uint32_t kKBytes = MKT * 128 * kHalves;
-  static constexpr uint32_t kQBytes = MQR * 128 * kHalves;
-  static constexpr uint32_t kKRing = DD == 128 ? 2 : 4;
-  static constexpr uint32_t kQRing = DD == 128 ? 2 : 4;
-  static constexpr uint32_t kBars = 1 + 2 * (kKRing + kQRing) + 8;
-  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + 16 + kMassLens * 4 + 8 * 64 * 8 + 2 * 128 * 4;
-  static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs per SM");
+  static constexpr uint32_t kQBytes = NQ * 128 * kHalves;
+  static constexpr uint32_t kKRing = kStream ? 2 : (DD == 64 ? 8 : (NQ == 64 ? 4 : (NQ == 32 ? 5 : 6)));
+  static constexpr uint32_t kQRing = kStream ? 4 : kKRing;
+  static constexpr uint32_t kRows = kStream ? 32 : NQ;    // columns of a warp
+  static constexpr uint32_t kBars = 2 * (kKRing + 2 * kQRing + kMassS) + 2;
+  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + kMassLens * 4 + kQRing * (2 * NQ + 4) * 4 + (kStream ? 2 * 3 * 128 * 4 : 0);
+  static_assert(kSmem <= 227 * 1024, "one CTA per SM");
 };
-constexpr uint32_t kMassS = 4;             // score buffers of 64 columns
 
 struct MassTcParams {
   MassArgs a;
-  uint32_t G, lt, rows, q_tiles, key_tiles, units, n_cols;
+  uint32_t G, lt, rows, q_tiles, units, items, n_cols;
   float scale_log2;
   unsigned int* err;
 };
@@ -53,15 +60,48 @@ __device__ __forceinline__ bool mass_wait(uint64_t* bar, uint32_t parity) {
   return true;
 }
 
-// (a0, a1) = (a0, a1) * s + (c0, c1) and (a0, a1) += (b0, b1) as packed instructions
-__device__ __forceinline__ void mass_fma2(float& a0, float& a1, float s, float c0, float c1) {
-  asm("{.reg .b64 ra, rb, rc;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %2};\n mov.b64 rc, {%3, %4};\n"
+// Packed fp32 pairs.
+struct F2 { float x, y; };
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("{.reg .b64 ra, rb, rc;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
       " fma.rn.f32x2 ra, ra, rb, rc;\n mov.b64 {%0, %1}, ra;}"
-      : "+f"(a0), "+f"(a1) : "f"(s), "f"(c0), "f"(c1));
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-__device__ __forceinline__ void mass_add2(float& a0, float& a1, float b0, float b1) {
-  asm("{.reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;}"
-      : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("{.reg .b64 ra, rb;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("{.reg .b64 ra, rb;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mul.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
+// x into [-126, 128], NaN kept: 2^x is then a normal number, or infinity at the upper end.
+__device__ __forceinline__ float ex2_range(float x) {
+  float y;
+  asm("{.reg .f32 t;\n max.NaN.f32 t, %1, 0fC2FC0000;\n min.NaN.f32 %0, t, 0f43000000;}" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^x of a pair without the special-function unit: x = n + f with n the nearest integer (adding 1.5 x 2^23 leaves it in the
+// low bits), 2^f by the polynomial of degree 5 with the least relative error on [-1/2, 1/2] (7.5e-8, 2.1e-7 as evaluated in fp32:
+// as exact as ex2.approx), times 2^n built in the exponent.
+__device__ __forceinline__ F2 ex2_fma(F2 v) {
+  const F2 x{ex2_range(v.x), ex2_range(v.y)};
+  const F2 t = add2(x, both(12582912.f));
+  const F2 f = fma2(add2(t, both(-12582912.f)), both(-1.f), x);
+  F2 r = fma2(both(0.0013276472454890609f), f, both(0.009675540961325169f));
+  r = fma2(r, f, both(0.05550713092088699f));
+  r = fma2(r, f, both(0.24022120237350464f));
+  r = fma2(r, f, both(0.6931469440460205f));
+  r = fma2(r, f, both(1.0000001192092896f));
+  const F2 s{__uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u)};
+  return mul2(r, s);
 }
 
 // One (batch, KV head, key tile) and the row tiles that can see it.
@@ -71,15 +111,16 @@ struct MassItem {
 
 __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t* lens_s, uint32_t round, MassItem& it) {
   // round r deals items r * grid .. in ascending or descending CTA order; key tiles ascend, so the work falls
-  const uint64_t id = uint64_t(round) * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-  if (id >= uint64_t(p.units) * p.key_tiles) return false;
-  const uint32_t kt = uint32_t(id / p.units), u = uint32_t(id % p.units);
+  const uint32_t id = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  if (round * gridDim.x >= p.items) return false;
+  if (id >= p.items) { it.qt0 = it.qt1 = 0; it.key0 = p.a.s; return true; }      // nothing in this round
+  const uint32_t kt = id / p.units, u = id % p.units;
   it.b = u / p.a.h_kv; it.kvh = u % p.a.h_kv; it.g = it.b % p.a.lens_n;
   it.key0 = kt * MKT;
   it.len = !p.a.kv_lens ? p.a.s : (it.g < kMassLens ? lens_s[it.g] : clamp_len(p.a.kv_lens[it.g], p.a.s));
   it.qt0 = 0;
   it.qt1 = it.key0 < it.len ? p.q_tiles : 0;
-  if (p.a.is_causal && !p.a.q_lens) {
+  if (p.q_tiles > 1 && p.a.is_causal && !p.a.q_lens) {
     // position i sees key0 when i >= key0 - (len - l)
     const int64_t first = int64_t(it.key0) - (int64_t(it.len) - int64_t(p.a.l));
     if (first > 0) it.qt0 = min(uint32_t(first) / p.lt, it.qt1);
@@ -88,11 +129,12 @@ __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t*
 }
 
 template <typename T, int DD, int NQ>
-__global__ void __launch_bounds__(kMassThreads<NQ>, 2)
+__global__ void __launch_bounds__(kMassThreads<NQ>, 1)
 attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const MassTcParams p) {
-  using MT = MassTile<DD>;
+  using MT = MassTile<DD, NQ>;
+  constexpr bool STREAM = MT::kStream;
   constexpr uint32_t KR = MT::kKRing, QR = MT::kQRing;
-  constexpr int GROUPS = kMassGroups<NQ>, THREADS = kMassThreads<NQ>;
+  constexpr uint32_t TMEM = kMassS * NQ;
   extern __shared__ __align__(1024) unsigned char smem[];
   if ((tc::smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicCAS(p.err, 0u, 50u);
@@ -105,37 +147,43 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* k_empty = k_full + KR;
   uint64_t* q_full = k_empty + KR;
   uint64_t* q_empty = q_full + QR;
-  uint64_t* s_full = q_empty + QR;       // kMassS
+  uint64_t* r_full = q_empty + QR;       // QR: log-sum-exp and limits of a tile's rows
+  uint64_t* r_empty = r_full + QR;
+  uint64_t* s_full = r_empty + QR;       // kMassS
   uint64_t* s_empty = s_full + kMassS;   // kMassS
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + kMassS);
-  uint32_t* lens_s = tmem_slot + 4;
-  float* row_s = reinterpret_cast<float*>(lens_s + kMassLens);            // per warp [2][32] -lse (log2 domain) and [2][32] limits
-  float* part_s = row_s + 8 * 128;                                         // [2][128] sums of the second group
+  uint32_t* lens_s = reinterpret_cast<uint32_t*>(bars + MT::kBars);
+  constexpr uint32_t RS = 2 * NQ + 4;    // words of a stage: -lse (log2 domain), limits, the least limit of each 32 rows
+  float* row_s = reinterpret_cast<float*>(lens_s + kMassLens);
+  float* part_s = row_s + QR * RS;       // [2][3][128] sums of the groups behind the first
   const MassArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tc::prefetch_tmap(&tmQ); tc::prefetch_tmap(&tmK);
     for (uint32_t i = 0; i < KR; ++i) { tc::mbar_init(&k_full[i], 1); tc::mbar_init(&k_empty[i], 1); }
-    for (uint32_t i = 0; i < QR; ++i) { tc::mbar_init(&q_full[i], 1); tc::mbar_init(&q_empty[i], 1); }
-    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], 4 * GROUPS); }
+    for (uint32_t i = 0; i < QR; ++i) {
+      tc::mbar_init(&q_full[i], 1); tc::mbar_init(&q_empty[i], 1);
+      tc::mbar_init(&r_full[i], kMassRowWarps<NQ>); tc::mbar_init(&r_empty[i], STREAM ? 4 * kMassGroups : 4);
+    }
+    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], STREAM ? 4 * kMassGroups : 4); }
     tc::fence_barrier_init();
   }
   if (warp == 1) {
-    tc::tmem_alloc(tmem_slot, kMassS * MQR);
+    tc::tmem_alloc(tmem_slot, TMEM);
     tc::tmem_relinquish();
   }
   if (p.rows < NQ) {
-    // rows of the tile that TMA does not fill feed columns nobody reads, but no stale bit patterns either
+    // rows of the tile that TMA does not fill feed columns nobody counts, but no stale bit patterns either
     const uint32_t per = (NQ - p.rows) * 8;
-    for (uint32_t i = threadIdx.x; i < per * QR * MT::kHalves; i += THREADS) {
+    for (uint32_t i = threadIdx.x; i < per * QR * MT::kHalves; i += kMassThreads<NQ>) {
       const uint32_t blk = i / per, o = i % per;         // blk = stage * halves + half
-      *reinterpret_cast<int4*>(q_s + blk * (MQR * 128) + p.rows * 128 + o * 16) = make_int4(0, 0, 0, 0);
+      *reinterpret_cast<int4*>(q_s + blk * (NQ * 128) + p.rows * 128 + o * 16) = make_int4(0, 0, 0, 0);
     }
     tc::fence_proxy_async();
   }
   pdl_wait();
   if (a.kv_lens)
-    for (uint32_t i = threadIdx.x; i < min(a.lens_n, kMassLens); i += THREADS) lens_s[i] = clamp_len(a.kv_lens[i], a.s);
+    for (uint32_t i = threadIdx.x; i < min(a.lens_n, kMassLens); i += kMassThreads<NQ>) lens_s[i] = clamp_len(a.kv_lens[i], a.s);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -163,7 +211,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           tc::mbar_expect_tx(&q_full[qb], MT::kHalves * p.rows * 128u);
 #pragma unroll
           for (uint32_t half = 0; half < MT::kHalves; ++half)
-            tc::tma_load_4d(q_s + qb * MT::kQBytes + half * (MQR * 128), &tmQ, &q_full[qb], int(half * 64), int(qt * p.lt), int(it.kvh * p.G), int(it.b));
+            tc::tma_load_4d(q_s + qb * MT::kQBytes + half * (NQ * 128), &tmQ, &q_full[qb], int(half * 64), int(qt * p.lt), int(it.kvh * p.G), int(it.b));
         }
       }
       // the copies in flight must land before the CTA leaves (they have, unless a wait ran out)
@@ -191,8 +239,8 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const uint64_t da = tc::make_smem_desc(ka + hh * (MKT * 128) + kk * 32, 16, 1024);
-              const uint64_t db = tc::make_smem_desc(qa + hh * (MQR * 128) + kk * 32, 16, 1024);
-              tc::umma_f16(tmem_base + sb * MQR, da, db, idesc, (hh | kk) ? 1u : 0u);
+              const uint64_t db = tc::make_smem_desc(qa + hh * (NQ * 128) + kk * 32, 16, 1024);
+              tc::umma_f16(tmem_base + sb * NQ, da, db, idesc, (hh | kk) ? 1u : 0u);
             }
           tc::umma_commit(&q_empty[qb]);
           tc::umma_commit(&s_full[sb]);
@@ -201,82 +249,137 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         ++nk;
       }
     }
+  } else if (warp >= 2 + 4 * kMassGroups) {
+    // ------------------------------ the rows' values: -lse and key limit, two tiles ahead -------
+    const uint32_t w = warp - (2 + 4 * kMassGroups), row = w * 32 + lane, gh = row / p.lt, ri = row - gh * p.lt;
+    const bool row_in = row < p.rows;
+    uint32_t round = 0, qt = 0;
+    bool more = true;
+    it.qt0 = it.qt1 = 0;
+    const float* lse_row = a.lse;
+    const int64_t* lim_row = a.q_lens;
+    struct Ahead { float lse; long long lim; uint32_t len; bool valid; };
+    auto fetch = [&]() {
+      Ahead f{0.f, 0, 0, false};
+      while (more && qt >= it.qt1) {
+        more = mass_item(p, lens_s, round++, it);
+        qt = it.qt0;
+        if (more && qt < it.qt1) {
+          lse_row = a.lse + (size_t(it.b) * a.h + it.kvh * p.G + gh) * a.l;
+          if (a.q_lens) lim_row = a.q_lens + size_t(it.g) * a.l;
+        }
+      }
+      if (!more) return f;
+      const uint32_t li = qt++ * p.lt + ri;
+      f.valid = true;
+      f.len = it.len;
+      if (row_in && li < a.l) {
+        f.lse = lse_row[li];
+        f.lim = a.q_lens ? lim_row[li] : (a.is_causal ? (long long)li + 1 + (long long)it.len - (long long)a.l : (long long)it.len);
+      }
+      return f;
+    };
+    Ahead f0 = fetch(), f1 = fetch();
+    for (uint32_t nq = 0; f0.valid; ++nq) {
+      const Ahead f2 = fetch();
+      const uint32_t qb = nq % QR;
+      if (nq >= QR && !__all_sync(0xffffffffu, mass_wait(&r_empty[qb], ((nq / QR) & 1) ^ 1))) { atomicCAS(p.err, 0u, 57u); break; }
+      float* rs = row_s + qb * RS;
+      float nl = -1.4426950408889634f * f0.lse;
+      uint32_t lim = clamp_len(f0.lim, f0.len);
+      if (isinf(nl)) { nl = 0.f; lim = 0; }                  // saw nothing, or is not to be counted
+      if (row < NQ) {
+        rs[row] = nl;
+        reinterpret_cast<uint32_t*>(rs)[NQ + row] = lim;
+      }
+      const uint32_t low = __reduce_min_sync(0xffffffffu, row < NQ ? lim : 0xffffffffu);
+      if (lane == 0) reinterpret_cast<uint32_t*>(rs)[2 * NQ + w] = low;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&r_full[qb]);
+      f0 = f1;
+      f1 = f2;
+    }
   } else {
     // ------------------------------ weights: one key per thread ---------------------------
+    constexpr uint32_t W = MT::kRows;                     // columns of this warp
+    constexpr uint32_t C = W < 32 ? W : 32;               // columns at a time
     const uint32_t quarter = warp & 3, key = quarter * 32 + lane, group = uint32_t(warp - 2) >> 2;
-    constexpr int W = NQ < 32 ? NQ : 32;                  // columns of this warp: group * 32 ..
-    const uint32_t s_base = tmem_base + ((quarter * 32) << 16) + group * 32;
-    float* nl_s = row_s + (warp - 2) * 128;
-    uint32_t* lim_s = reinterpret_cast<uint32_t*>(nl_s + 64);
-    const uint32_t row = group * 32 + lane, gh = row / p.lt, ri = row % p.lt;      // the row this lane looks after
-    const bool row_in = row < p.rows;
-    uint32_t nq = 0, n_item = 0;
+    const uint32_t col0 = STREAM ? group * 32 : 0;
+    const uint32_t s_base = tmem_base + ((quarter * 32) << 16) + col0;
     bool ok = true;
+    uint32_t tile = 0, n_item = 0;
     for (uint32_t round = 0; mass_item(p, lens_s, round, it); ++round) {
       const uint32_t j = it.key0 + key;
-      float total = 0.f;
-      // -lse and limit of the lane's row, one tile ahead
-      float nl = 0.f;
-      uint32_t lim = 0;
-      const float* lse_row = a.lse + (size_t(it.b) * a.h + it.kvh * p.G + gh) * a.l;
-      auto fetch = [&](uint32_t qt) {
-        const uint32_t li = qt * p.lt + ri;
-        nl = 0.f; lim = 0;
-        if (row_in && qt < it.qt1 && li < a.l) {
-          nl = -1.4426950408889634f * lse_row[li];
-          if (a.q_lens) lim = clamp_len(a.q_lens[size_t(it.g) * a.l + li], it.len);
-          else if (a.is_causal) lim = clamp_len((long long)li + 1 + (long long)it.len - (long long)a.l, it.len);
-          else lim = it.len;
-        }
-      };
-      fetch(it.qt0);
+      const bool any = it.qt0 < it.qt1;
+      // without row tiles a round is dealt by its number, with one by the tile's: a group waits for every use of its score buffer
+      // in turn
+      if (!STREAM && (any ? tile++ : round) % kMassGroups != group) continue;
+      const size_t o = (size_t(it.b) * a.h_kv + it.kvh) * a.s + j;
+      float total = 0.f, old = 0.f;
+      if (!STREAM && a.mass && j < a.s) old = a.mass[o];
+      uint32_t nq = STREAM ? tile : tile - 1;
       for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
-        const uint32_t buf = (nq & 1) * 32, sb = nq % kMassS;
-        if (isinf(nl)) { nl = 0.f; lim = 0; }             // saw nothing, or is not to be counted
-        nl_s[buf + lane] = nl;
-        lim_s[buf + lane] = lim;
-        const bool all = __all_sync(0xffffffffu, lim >= it.key0 + MKT);      // every row counts for every key of the tile
-        fetch(qt + 1);
-        if (ok && !__all_sync(0xffffffffu, mass_wait(&s_full[sb], (nq / kMassS) & 1))) { atomicCAS(p.err, 0u, 56u); ok = false; }
+        const uint32_t sb = nq % kMassS, qb = nq % QR;
+        if (ok && !__all_sync(0xffffffffu, mass_wait(&r_full[qb], (nq / QR) & 1) && mass_wait(&s_full[sb], (nq / kMassS) & 1))) {
+          atomicCAS(p.err, 0u, 56u);
+          ok = false;
+        }
         tc::tc_fence_after();
-        float sv[W];
-        if constexpr (W == 16) tc::tmem_ld16(s_base + sb * MQR, sv);
-        else tc::tmem_ld32(s_base + sb * MQR, sv);
-        tc::tmem_ld_wait();
-        tc::tc_fence_before();
-        __syncwarp();                                      // the row's values are in place, too
-        if (lane == 0) tc::mbar_arrive(&s_empty[sb]);
-        float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
-        if (all) {
+        const float* rs = row_s + qb * RS;
+        float part = 0.f;
 #pragma unroll
-          for (int c = 0; c < W; c += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(nl_s + buf + c);
-            mass_fma2(sv[c], sv[c + 1], p.scale_log2, x.x, x.y);
-            mass_fma2(sv[c + 2], sv[c + 3], p.scale_log2, x.z, x.w);
-            mass_add2(r0, r1, fast_ex2(sv[c]), fast_ex2(sv[c + 1]));
-            mass_add2(r2, r3, fast_ex2(sv[c + 2]), fast_ex2(sv[c + 3]));
+        for (uint32_t h = 0; h < W / C; ++h) {
+          float sv[C];
+          if constexpr (C == 16) tc::tmem_ld16(s_base + sb * NQ, sv);
+          else tc::tmem_ld32(s_base + sb * NQ + h * C, sv);
+          tc::tmem_ld_wait();
+          if (h == W / C - 1) {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s_empty[sb]);
           }
-        } else {
+          const float* nlc = rs + col0 + h * C;
+          const uint32_t* lmc = reinterpret_cast<const uint32_t*>(rs) + NQ + col0 + h * C;
+          if (reinterpret_cast<const uint32_t*>(rs)[2 * NQ + (col0 + h * C) / 32] >= it.key0 + MKT) {
+            // every row counts for every key of the tile
+            F2 r0 = both(0.f), r1 = both(0.f);
 #pragma unroll
-          for (int c = 0; c < W; ++c) {
-            const float w = fast_ex2(fmaf(sv[c], p.scale_log2, nl_s[buf + c]));
-            r0 += j < lim_s[buf + c] ? w : 0.f;
+            for (uint32_t c = 0; c < C; c += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(nlc + c);
+              const F2 u = fma2(F2{sv[c], sv[c + 1]}, both(p.scale_log2), F2{x.x, x.y});
+              const F2 v = fma2(F2{sv[c + 2], sv[c + 3]}, both(p.scale_log2), F2{x.z, x.w});
+              // pairs 1 and 5 of eight by the polynomial
+              constexpr uint32_t kPoly = STREAM ? 0x22u : 0u;
+              r0 = add2(r0, (kPoly >> (c / 2 % 8)) & 1u ? ex2_fma(u) : F2{fast_ex2(u.x), fast_ex2(u.y)});
+              r1 = add2(r1, (kPoly >> ((c / 2 + 1) % 8)) & 1u ? ex2_fma(v) : F2{fast_ex2(v.x), fast_ex2(v.y)});
+            }
+            r0 = add2(r0, r1);
+            part += r0.x + r0.y;
+          } else {
+#pragma unroll
+            for (uint32_t c = 0; c < C; ++c) {
+              const float w = fast_ex2(fmaf(sv[c], p.scale_log2, nlc[c]));
+              part += j < lmc[c] ? w : 0.f;
+            }
           }
         }
-        total += (r0 + r1) + (r2 + r3);
+        total += part;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&r_empty[qb]);
       }
-      if constexpr (GROUPS == 2) {
-        // the second group's sums come through shared memory; two buffers and one meeting per item: a thread that is an item
-        // ahead writes the other buffer
-        float* part = part_s + (n_item++ & 1) * 128;
-        if (group == 1) part[key] = total;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (group == 0) total += part[key];
+      if constexpr (STREAM) {
+        if (any) {
+          // the other groups' sums come through shared memory, added in group order; two buffers and one meeting per item: a
+          // thread that is an item ahead writes the other buffer
+          tile = nq;
+          float* part = part_s + (n_item++ & 1) * 384;
+          if (group > 0) part[(group - 1) * 128 + key] = total;
+          asm volatile("bar.sync 1, 512;" ::: "memory");
+          if (group == 0) total += part[key] + part[128 + key] + part[256 + key];
+        }
+        if (group == 0 && a.mass && j < a.s) old = a.mass[o];
       }
-      if (group == 0 && j < a.s) {
-        const size_t o = (size_t(it.b) * a.h_kv + it.kvh) * a.s + j;
-        if (a.mass != a.out || j < it.len) a.out[o] = (a.mass ? a.mass[o] : 0.f) + (j < it.len ? total : 0.f);
-      }
+      if ((!STREAM || group == 0) && j < a.s && (a.mass != a.out || j < it.len)) a.out[o] = old + (j < it.len ? total : 0.f);
     }
   }
   tc::tc_fence_before();
@@ -284,13 +387,14 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == 1) {
     __syncwarp();
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem_base, kMassS * MQR);
+    tc::tmem_dealloc(tmem_base, TMEM);
   }
 }
 
 bool attn_mass_tc_eligible(const MassArgs& a) {
   if (a.dtype != KUIOPS_BF16 && a.dtype != KUIOPS_F16) return false;
-  if (a.e > 128 || a.e % 8 || a.h / a.h_kv > MQR) return false;
+  if (a.e > 128 || a.e % 8 || a.h / a.h_kv > 128) return false;
+  if (uint64_t(a.n) * a.h_kv * ((a.s + MKT - 1) / MKT) >= (1ull << 31)) return false;
   auto ok = [&](const void* t, int64_t sn, int64_t sh, int64_t sl, uint32_t heads, uint32_t rows) {
     auto st = [](int64_t s) { return s > 0 && s % 8 == 0 && uint64_t(s) * 2 < (1ull << 40); };
     return aligned16(t) && (rows == 1 || st(sl)) && (heads == 1 || st(sh)) && (a.n == 1 || st(sn));
@@ -301,7 +405,7 @@ bool attn_mass_tc_eligible(const MassArgs& a) {
 template <typename T, int DD, int NQ>
 static int mass_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const MassTcParams& p, cudaStream_t st) {
   auto kern = attn_mass_tc_kernel<T, DD, NQ>;
-  constexpr size_t smem = MassTile<DD>::kSmem;
+  constexpr size_t smem = MassTile<DD, NQ>::kSmem;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KUIOPS_ELAUNCH;
@@ -310,30 +414,31 @@ static int mass_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const Ma
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return KUIOPS_ELAUNCH;
     configured.fetch_or(bit, std::memory_order_release);
   }
-  const uint64_t items = uint64_t(p.units) * p.key_tiles, slots = 2ull * num_sms();
-  return launch_pdl(kern, dim3(unsigned(items < slots ? items : slots)), dim3(kMassThreads<NQ>), smem, st, mq, mk, p);
+  const uint32_t slots = uint32_t(num_sms());
+  return launch_pdl(kern, dim3(p.items < slots ? p.items : slots), dim3(kMassThreads<NQ>), smem, st, mq, mk, p);
 }
 
 template <typename T, int DD>
-static int mass_tc_launch_rows(const CUtensorMap& mq, const CUtensorMap& mk, MassTcParams& p, cudaStream_t st) {
-  p.n_cols = (p.rows + 15) & ~15u;
-  if (p.rows <= 16) return mass_tc_launch<T, DD, 16>(mq, mk, p, st);
-  if (p.rows <= 32) return mass_tc_launch<T, DD, 32>(mq, mk, p, st);
-  return mass_tc_launch<T, DD, 64>(mq, mk, p, st);
+static int mass_tc_launch_rows(const CUtensorMap& mq, const CUtensorMap& mk, const MassTcParams& p, uint32_t nq, cudaStream_t st) {
+  if (nq == 16) return mass_tc_launch<T, DD, 16>(mq, mk, p, st);
+  if (nq == 32) return mass_tc_launch<T, DD, 32>(mq, mk, p, st);
+  if (nq == 64) return mass_tc_launch<T, DD, 64>(mq, mk, p, st);
+  return mass_tc_launch<T, DD, 128>(mq, mk, p, st);
 }
 
 int attn_mass_tc(const MassArgs& a, cudaStream_t st) {
   MassTcParams p = {};
   p.a = a; p.G = a.h / a.h_kv;
+  const uint64_t all = uint64_t(p.G) * a.l;
+  const uint32_t nq = all <= 16 ? 16 : (all <= 32 ? 32 : (all <= 64 ? 64 : 128));
   // as few row tiles as hold all rows, of even size
-  p.q_tiles = (a.l + MQR / p.G - 1) / (MQR / p.G);
+  p.q_tiles = (a.l + nq / p.G - 1) / (nq / p.G);
   p.lt = (a.l + p.q_tiles - 1) / p.q_tiles;
   p.q_tiles = (a.l + p.lt - 1) / p.lt;
   p.rows = p.G * p.lt;
-  p.key_tiles = (a.s + MKT - 1) / MKT;
-  const uint64_t units = uint64_t(a.n) * a.h_kv;
-  if (units >= (1ull << 31)) return KUIOPS_ELIMIT;
-  p.units = uint32_t(units);
+  p.n_cols = (p.rows + 15) & ~15u;
+  p.units = a.n * a.h_kv;
+  p.items = p.units * ((a.s + MKT - 1) / MKT);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = tc_error_word_device();
   if (!p.err) return KUIOPS_ELAUNCH;
@@ -350,8 +455,8 @@ int attn_mass_tc(const MassArgs& a, cudaStream_t st) {
   if (!enc(&mq, a.Q, a.l, a.h, a.q_sn, a.q_sh, a.q_sl, p.lt, p.G)) return KUIOPS_EDRIVER;
   if (!enc(&mk, a.K, a.s, a.h_kv, a.k_sn, a.k_sh, a.k_ss, MKT, 1)) return KUIOPS_EDRIVER;
   if (a.dtype == KUIOPS_BF16)
-    return a.e > 64 ? mass_tc_launch_rows<__nv_bfloat16, 128>(mq, mk, p, st) : mass_tc_launch_rows<__nv_bfloat16, 64>(mq, mk, p, st);
-  return a.e > 64 ? mass_tc_launch_rows<__half, 128>(mq, mk, p, st) : mass_tc_launch_rows<__half, 64>(mq, mk, p, st);
+    return a.e > 64 ? mass_tc_launch_rows<__nv_bfloat16, 128>(mq, mk, p, nq, st) : mass_tc_launch_rows<__nv_bfloat16, 64>(mq, mk, p, nq, st);
+  return a.e > 64 ? mass_tc_launch_rows<__half, 128>(mq, mk, p, nq, st) : mass_tc_launch_rows<__half, 64>(mq, mk, p, nq, st);
 }
 
 }  // namespace kuiops
