@@ -11,9 +11,9 @@
 //   latencies (log-sum-exp, scores, the old mass) hide behind three other items.
 //   More rows (a window, a prompt): bound by the exponentials, 16 per clock and SM, then by the products.  Tiles of 128 rows
 //   stream past a resident K tile (128 columns: a 64-column product would be bound by shared memory, whose A operand it reads
-//   twice as often) and every group takes 32 columns of each.  A quarter of the exponentials is made by a polynomial in the FMA
-//   pipe instead of the special-function unit.  Items are dealt in alternating direction, which evens out a causal
-//   mask's falling work per item.
+//   twice as often) and every group takes 32 columns of each.  Items are dealt in alternating direction, which evens out a causal mask's
+//   falling work per item.  (Making a quarter of the exponentials by a polynomial in the FMA pipe was slower, 396 against
+//   361 us for an 8192-token prompt: the instructions it takes are what the scheduler has least of.)
 #include "tree.cuh"
 #include "tc_ptx.cuh"
 #include <type_traits>
@@ -42,9 +42,23 @@ template <int DD, int NQ> struct MassTile {
   static_assert(kSmem <= 227 * 1024, "one CTA per SM");
 };
 
+// Division of a 31-bit number by a launch constant: q = (umulhi(n, mul) + n) >> shift with 2^(shift - 1) < d <= 2^shift
+// and mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery, "Division by invariant integers using
+// multiplication", 1994).  The hardware has no integer division; its sequence was most of an item's cost here.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  void set(uint32_t v) {
+    d = v;
+    for (shift = 0; (1ull << shift) < v; ++shift) {}
+    mul = uint32_t((((1ull << shift) - v) << 32) / v + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct MassTcParams {
   MassArgs a;
-  uint32_t G, lt, rows, q_tiles, units, items, n_cols;
+  uint32_t G, lt, rows, q_tiles, items, n_cols;
+  FastDiv by_item, by_heads, by_lens, by_lt;      // adjacent items, KV heads, key counts, positions per row tile
   float scale_log2;
   unsigned int* err;
 };
@@ -75,47 +89,23 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("{.reg .b64 ra, rb;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mul.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra;}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 __device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
-// x into [-126, 128], NaN kept: 2^x is then a normal number, or infinity at the upper end.
-__device__ __forceinline__ float ex2_range(float x) {
-  float y;
-  asm("{.reg .f32 t;\n max.NaN.f32 t, %1, 0fC2FC0000;\n min.NaN.f32 %0, t, 0f43000000;}" : "=f"(y) : "f"(x));
-  return y;
-}
-// 2^x of a pair without the special-function unit: x = n + f with n the nearest integer (adding 1.5 x 2^23 leaves it in the
-// low bits), 2^f by the polynomial of degree 5 with the least relative error on [-1/2, 1/2] (7.5e-8, 2.1e-7 as evaluated in fp32:
-// as exact as ex2.approx), times 2^n built in the exponent.
-__device__ __forceinline__ F2 ex2_fma(F2 v) {
-  const F2 x{ex2_range(v.x), ex2_range(v.y)};
-  const F2 t = add2(x, both(12582912.f));
-  const F2 f = fma2(add2(t, both(-12582912.f)), both(-1.f), x);
-  F2 r = fma2(both(0.0013276472454890609f), f, both(0.009675540961325169f));
-  r = fma2(r, f, both(0.05550713092088699f));
-  r = fma2(r, f, both(0.24022120237350464f));
-  r = fma2(r, f, both(0.6931469440460205f));
-  r = fma2(r, f, both(1.0000001192092896f));
-  const F2 s{__uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u)};
-  return mul2(r, s);
-}
-
 // One (batch, KV head, key tile) and the row tiles that can see it.
 struct MassItem {
   uint32_t b, kvh, g, key0, len, qt0, qt1;
 };
 
 __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t* lens_s, uint32_t round, MassItem& it) {
-  // round r deals items r * grid .. in ascending or descending CTA order; key tiles ascend, so the work falls
+  // Round r deals items r * grid .. in ascending or descending CTA order.  With several row tiles the key tiles come first, so
+  // that a causal mask's work falls with the item; with one the CTAs of a round read adjacent keys.
   const uint32_t id = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   if (round * gridDim.x >= p.items) return false;
   if (id >= p.items) { it.qt0 = it.qt1 = 0; it.key0 = p.a.s; return true; }      // nothing in this round
-  const uint32_t kt = id / p.units, u = id % p.units;
-  it.b = u / p.a.h_kv; it.kvh = u % p.a.h_kv; it.g = it.b % p.a.lens_n;
+  const uint32_t hi = p.by_item.div(id), lo = id - hi * p.by_item.d;
+  const uint32_t kt = p.q_tiles > 1 ? hi : lo, u = p.q_tiles > 1 ? lo : hi;
+  it.b = p.by_heads.div(u);
+  it.kvh = u - it.b * p.a.h_kv;
+  it.g = it.b - p.by_lens.div(it.b) * p.a.lens_n;
   it.key0 = kt * MKT;
   it.len = !p.a.kv_lens ? p.a.s : (it.g < kMassLens ? lens_s[it.g] : clamp_len(p.a.kv_lens[it.g], p.a.s));
   it.qt0 = 0;
@@ -123,7 +113,7 @@ __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t*
   if (p.q_tiles > 1 && p.a.is_causal && !p.a.q_lens) {
     // position i sees key0 when i >= key0 - (len - l)
     const int64_t first = int64_t(it.key0) - (int64_t(it.len) - int64_t(p.a.l));
-    if (first > 0) it.qt0 = min(uint32_t(first) / p.lt, it.qt1);
+    if (first > 0) it.qt0 = min(p.by_lt.div(uint32_t(first)), it.qt1);
   }
   return true;
 }
@@ -223,25 +213,27 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     if (lane == 0) {
       constexpr int is_bf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       const uint32_t idesc = tc::make_idesc(is_bf16, 0, 0, MKT, int(p.n_cols));
+      // a descriptor's low bits are the address in 16-byte units: stages and steps are additions
+      const uint64_t k_desc0 = tc::make_smem_desc(tc::smem_u32(k_s), 16, 1024), q_desc0 = tc::make_smem_desc(tc::smem_u32(q_s), 16, 1024);
       uint32_t nk = 0, nq = 0;
       bool ok = true;
       for (uint32_t round = 0; ok && mass_item(p, lens_s, round, it); ++round) {
         if (it.qt0 >= it.qt1) continue;
-        const uint32_t kb = nk % KR, ka = tc::smem_u32(k_s + kb * MT::kKBytes);
+        const uint32_t kb = nk % KR;
+        const uint64_t k_desc = k_desc0 + kb * (MT::kKBytes >> 4);
         if (!mass_wait(&k_full[kb], (nk / KR) & 1)) { atomicCAS(p.err, 0u, 53u); break; }
         for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
-          const uint32_t qb = nq % QR, sb = nq % kMassS, qa = tc::smem_u32(q_s + qb * MT::kQBytes);
+          const uint32_t qb = nq % QR, sb = nq % kMassS;
+          const uint64_t q_desc = q_desc0 + qb * (MT::kQBytes >> 4);
           if (!mass_wait(&q_full[qb], (nq / QR) & 1)) { atomicCAS(p.err, 0u, 54u); ok = false; break; }
           if (nq >= kMassS && !mass_wait(&s_empty[sb], ((nq / kMassS) & 1) ^ 1)) { atomicCAS(p.err, 0u, 55u); ok = false; break; }
           tc::tc_fence_after();
 #pragma unroll
           for (uint32_t hh = 0; hh < MT::kHalves; ++hh)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t da = tc::make_smem_desc(ka + hh * (MKT * 128) + kk * 32, 16, 1024);
-              const uint64_t db = tc::make_smem_desc(qa + hh * (NQ * 128) + kk * 32, 16, 1024);
-              tc::umma_f16(tmem_base + sb * NQ, da, db, idesc, (hh | kk) ? 1u : 0u);
-            }
+            for (int kk = 0; kk < 4; ++kk)
+              tc::umma_f16(tmem_base + sb * NQ, k_desc + (hh * (MKT * 128) + kk * 32) / 16, q_desc + (hh * (NQ * 128) + kk * 32) / 16, idesc,
+                           (hh | kk) ? 1u : 0u);
           tc::umma_commit(&q_empty[qb]);
           tc::umma_commit(&s_full[sb]);
         }
@@ -316,7 +308,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (!STREAM && (any ? tile++ : round) % kMassGroups != group) continue;
       const size_t o = (size_t(it.b) * a.h_kv + it.kvh) * a.s + j;
       float total = 0.f, old = 0.f;
-      if (!STREAM && a.mass && j < a.s) old = a.mass[o];
+      if ((!STREAM || group == 0) && a.mass && j < a.s) old = a.mass[o];
       uint32_t nq = STREAM ? tile : tile - 1;
       for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
         const uint32_t sb = nq % kMassS, qb = nq % QR;
@@ -348,10 +340,8 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               const float4 x = *reinterpret_cast<const float4*>(nlc + c);
               const F2 u = fma2(F2{sv[c], sv[c + 1]}, both(p.scale_log2), F2{x.x, x.y});
               const F2 v = fma2(F2{sv[c + 2], sv[c + 3]}, both(p.scale_log2), F2{x.z, x.w});
-              // pairs 1 and 5 of eight by the polynomial
-              constexpr uint32_t kPoly = STREAM ? 0x22u : 0u;
-              r0 = add2(r0, (kPoly >> (c / 2 % 8)) & 1u ? ex2_fma(u) : F2{fast_ex2(u.x), fast_ex2(u.y)});
-              r1 = add2(r1, (kPoly >> ((c / 2 + 1) % 8)) & 1u ? ex2_fma(v) : F2{fast_ex2(v.x), fast_ex2(v.y)});
+              r0 = add2(r0, F2{fast_ex2(u.x), fast_ex2(u.y)});
+              r1 = add2(r1, F2{fast_ex2(v.x), fast_ex2(v.y)});
             }
             r0 = add2(r0, r1);
             part += r0.x + r0.y;
@@ -377,7 +367,6 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           asm volatile("bar.sync 1, 512;" ::: "memory");
           if (group == 0) total += part[key] + part[128 + key] + part[256 + key];
         }
-        if (group == 0 && a.mass && j < a.s) old = a.mass[o];
       }
       if ((!STREAM || group == 0) && j < a.s && (a.mass != a.out || j < it.len)) a.out[o] = old + (j < it.len ? total : 0.f);
     }
@@ -437,8 +426,12 @@ int attn_mass_tc(const MassArgs& a, cudaStream_t st) {
   p.q_tiles = (a.l + p.lt - 1) / p.lt;
   p.rows = p.G * p.lt;
   p.n_cols = (p.rows + 15) & ~15u;
-  p.units = a.n * a.h_kv;
-  p.items = p.units * ((a.s + MKT - 1) / MKT);
+  const uint32_t units = a.n * a.h_kv, key_tiles = (a.s + MKT - 1) / MKT;
+  p.items = units * key_tiles;
+  p.by_item.set(p.q_tiles > 1 ? units : key_tiles);
+  p.by_heads.set(a.h_kv);
+  p.by_lens.set(a.lens_n);
+  p.by_lt.set(p.lt);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = tc_error_word_device();
   if (!p.err) return KUIOPS_ELAUNCH;

@@ -184,20 +184,20 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       constexpr uint32_t idesc_pv = tc::make_idesc(is_bf16, 0, 1, 128, DD);
       bool ok = tree_wait(q_full, 0);
       if (!ok) atomicCAS(p.err, 0u, 42u);
-      const uint32_t qa = tc::smem_u32(q_s);
+      // a descriptor's low bits are the address in 16-byte units: tiles and steps are additions
+      const uint64_t q_desc = tc::make_smem_desc(tc::smem_u32(q_s), 16, 1024), k_desc0 = tc::make_smem_desc(tc::smem_u32(ring), 16, 1024);
+      const uint64_t v_desc0 = tc::make_smem_desc(tc::smem_u32(ring), RTN * 128, 1024);
       auto issue_qk = [&](uint32_t j) -> bool {
         const uint32_t n = 2 * j, buf = n % R;
-        const uint32_t ka = tc::smem_u32(ring + buf * TT::kTBytes);
+        const uint64_t k_desc = k_desc0 + buf * (TT::kTBytes >> 4);
         if (!tree_wait(&t_full[buf], (n / R) & 1)) { atomicCAS(p.err, 0u, 43u); return false; }
         tc::tc_fence_after();
 #pragma unroll
         for (uint32_t hh = 0; hh < TT::kHalves; ++hh)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t da = tc::make_smem_desc(qa + hh * (128 * 128) + kk * 32, 16, 1024);
-            const uint64_t db = tc::make_smem_desc(ka + hh * (RTN * 128) + kk * 32, 16, 1024);
-            tc::umma_f16(tmem_S + (j & 1) * RTN, da, db, idesc_qk, (hh | kk) ? 1u : 0u);
-          }
+          for (int kk = 0; kk < 4; ++kk)
+            tc::umma_f16(tmem_S + (j & 1) * RTN, q_desc + (hh * (128 * 128) + kk * 32) / 16, k_desc + (hh * (RTN * 128) + kk * 32) / 16, idesc_qk,
+                         (hh | kk) ? 1u : 0u);
         tc::umma_commit(&t_empty[buf]);
         tc::umma_commit(&s_full[j & 1]);
         return true;
@@ -205,7 +205,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (ok) ok = issue_qk(0);
       for (uint32_t j = 0; j < n_tiles && ok; ++j) {
         const uint32_t n = 2 * j + 1, buf = n % R;
-        const uint32_t va = tc::smem_u32(ring + buf * TT::kTBytes);
+        const uint64_t v_desc = v_desc0 + buf * (TT::kTBytes >> 4);
         // The next tile's scores are computed during this tile's softmax.  Their buffer holds P of tile j - 1, whose
         // product was issued before (the pipe runs in order), and the softmax left it when p_ready of j - 1 arrived.
         if (j + 1 < n_tiles && !issue_qk(j + 1)) { ok = false; break; }
@@ -213,10 +213,8 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (!tree_wait(&t_full[buf], (n / R) & 1)) { atomicCAS(p.err, 0u, 45u); ok = false; break; }
         tc::tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint64_t db = tc::make_smem_desc(va + kk * 2048, RTN * 128, 1024);
-          tc::umma_f16_ts(tmem_O, tmem_S + (j & 1) * RTN + kk * 8, db, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < 4; ++kk)
+          tc::umma_f16_ts(tmem_O, tmem_S + (j & 1) * RTN + kk * 8, v_desc + kk * 128, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
         tc::umma_commit(&t_empty[buf]);
         tc::umma_commit(o_done);
       }
