@@ -42,19 +42,6 @@ template <int DD, int NQ> struct MassTile {
   static_assert(kSmem <= 227 * 1024, "one CTA per SM");
 };
 
-// Division of a 31-bit number by a launch constant: q = (umulhi(n, mul) + n) >> shift with 2^(shift - 1) < d <= 2^shift
-// and mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery, "Division by invariant integers using
-// multiplication", 1994).  The hardware has no integer division; its sequence was most of an item's cost here.
-struct FastDiv {
-  uint32_t d, mul, shift;
-  void set(uint32_t v) {
-    d = v;
-    for (shift = 0; (1ull << shift) < v; ++shift) {}
-    mul = uint32_t((((1ull << shift) - v) << 32) / v + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
 struct MassTcParams {
   MassArgs a;
   uint32_t G, lt, rows, q_tiles, items, n_cols;

@@ -276,6 +276,8 @@ static size_t tree_record_bytes(const TreeArgs& a, uint32_t splits) {
   return splits <= 1 ? 0 : size_t(a.n) * a.h * a.l * splits * tree_record_floats(a.ev) * sizeof(float);
 }
 
+static bool tree_tc_shape(const TreeArgs& a) { return a.dtype != KUIOPS_F32 && a.e <= 128 && a.ev <= 128 && a.h / a.h_kv <= 128; }
+
 extern "C" {
 
 size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e,
@@ -284,9 +286,8 @@ size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint3
   if (tree_shape(dtype, n, h, h_kv, l, s, e, ev) != KUIOPS_OK) return 0;
   a.dtype = dtype; a.n = n; a.h = h; a.h_kv = h_kv; a.l = l; a.s = s; a.e = e; a.ev = ev;
   // which kernel runs also depends on alignment, unknown here: cover both
-  const uint32_t simt = sdpa_tree_simt_splits(a);
-  const uint32_t tc = dtype != KUIOPS_F32 && e <= 128 && ev <= 128 && h / h_kv <= 128 ? sdpa_tree_tc_splits(a) : 1;
-  return tree_record_bytes(a, simt > tc ? simt : tc);
+  const size_t simt = tree_record_bytes(a, sdpa_tree_simt_splits(a)), tc = tree_tc_shape(a) ? sdpa_tree_tc_workspace_bytes(a) : 0;
+  return simt > tc ? simt : tc;
 }
 
 int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream) {
@@ -302,10 +303,12 @@ int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream) 
   if (!(a.scale - a.scale == 0.f)) return KUIOPS_EINVAL;          // a finite number
   cudaStream_t st = as_stream(stream);
   const bool tc = sdpa_tree_tc_eligible(a);
-  const uint32_t splits = tc ? sdpa_tree_tc_splits(a) : sdpa_tree_simt_splits(a);
-  if (splits > 1 && (!a.workspace || a.workspace_bytes < tree_record_bytes(a, splits) || !aligned16(a.workspace))) return KUIOPS_EWORKSPACE;
+  const uint32_t splits = sdpa_tree_simt_splits(a);
+  const size_t need = tc ? sdpa_tree_tc_workspace_bytes(a) : tree_record_bytes(a, splits);
+  if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace))) return KUIOPS_EWORKSPACE;
+  if (tc) return sdpa_tree_tc(a, st);
   float* partials = static_cast<float*>(a.workspace);
-  const int run = tc ? sdpa_tree_tc(a, partials, st) : sdpa_tree_simt(a, partials, splits, st);
+  const int run = sdpa_tree_simt(a, partials, splits, st);
   if (run != KUIOPS_OK || splits == 1) return run;
   return sdpa_tree_merge(a, partials, splits, st);
 }

@@ -570,6 +570,17 @@ def _elsewhere(dev, what, *tensors):
     return None if dev == (_cur_device() if _cur_device is not None else torch.cuda.current_device()) else torch.cuda.device(dev)
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _buffer(kind, device, nbytes):
+    """Scratch without initial contents.  Eager calls on a stream share theirs; a captured call gets its own, because two graphs
+    captured on one stream may be replayed side by side."""
+    if _capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return workspace(kind, device, nbytes)
+
+
 def _rows_last(t):
     """Strides of a 4-D tensor whose innermost dimension is contiguous and whose rows do not overlap (a copy of it otherwise)."""
     a, b, c, d = t.stride()
@@ -636,8 +647,7 @@ def sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, *, scale=None, need_lse=True, out=
     L = lib()
     code = dtype_code(dt)
     wsb = L.kuiops_sdpa_tree_workspace_bytes(code, n, h, hkv, l, s, e, ev)
-    # a buffer of this call alone: captured graphs keep theirs, and calls on several streams do not meet
-    ws = torch.empty(wsb, dtype=torch.uint8, device=out.device) if wsb else None
+    ws = _buffer("sdpa_tree", out.device, wsb) if wsb else None
     _check(L.kuiops_sdpa_tree(_TREE_ARGS.pack(
         Q.data_ptr(), K.data_ptr(), V.data_ptr(), Kd.data_ptr(), Vd.data_ptr(), mask.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr(),

@@ -123,7 +123,8 @@ def test_contracts_of_the_c_entries():
     L = _ffi.lib()
     for name in ("sdpa_tree", "kv_append", "attn_mass", "kv_evict"):
         assert getattr(L, "kuiops_" + name)(None, None) == _ffi.EINVAL
-    tree = c_call("sdpa_tree", dict(dtype=_ffi.BF16, n=1, h=4, h_kv=2, l=3, s=10, e=128, ev=128, Q=P, K=P, V=P, DK=P, DV=P, mask=P, out=P, workspace=P,
+    tree = c_call("sdpa_tree", dict(dtype=_ffi.BF16, n=1, h=4, h_kv=2, l=3, s=10, e=128, ev=128, q_sn=8, q_sh=128, k_sn=8, k_sh=128, v_sn=8, v_sh=128, dk_sh=128, dv_sh=128,
+                                    o_sh=128, Q=P, K=P, V=P, DK=P, DV=P, mask=P, out=P, workspace=P,
                                     workspace_bytes=1 << 30, q_sl=128, k_ss=128, v_ss=128, dk_sl=128, dv_sl=128, o_sl=128, scale=0.1))
     assert tree(dtype=7) == tree(n=0) == tree(l=0) == tree(h=3) == tree(Q=0) == tree(K=0) == tree(mask=0) == tree(out=0) == _ffi.EINVAL
     assert tree(k_ss=64) == tree(mask_sn=8) == tree(scale=float("nan")) == tree(scale=float("inf")) == _ffi.EINVAL
@@ -211,12 +212,19 @@ TREE_CASES = [
     (1, 8, 2, 9, 1500, 64, [1400], "f32"),
     (1, 2, 2, 5, 40, 24, [0], "f32"),
     (1, 160, 1, 2, 70, 128, [65], "bf16"),              # more heads per KV head than a tile has rows
+    # more units than CTAs: a CTA walks several, ends in the middle of one and goes on in the middle of another
+    (80, 8, 8, 2, 260, 128, [(i * 37) % 261 for i in range(80)], "bf16"),
+    (60, 16, 8, 12, 130, 64, [(i * 53) % 131 for i in range(60)], "f16"),
+    (40, 16, 8, 24, 200, 128, [(i * 29) % 201 for i in range(40)], "bf16"),
+    (24, 64, 8, 12, 300, 128, [300 - (i * 41) % 299 for i in range(24)], "bf16"),
+    (18, 16, 2, 33, 700, 128, [(i * 97) % 701 for i in range(18)], "f16"),     # three tiles of rows
+    (300, 2, 1, 1, 70, 128, [i % 71 for i in range(300)], "bf16"),
 ]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("masks", ["tree", "random"])
-@pytest.mark.parametrize("case", TREE_CASES, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
+@pytest.mark.parametrize("case", TREE_CASES, ids=lambda c: "-".join(str(x) for x in c[:6] + c[7:] + (c[6][:3],)).replace(" ", ""))
 def test_tree_attention(cuda, case, masks):
     n, h, hk, l, s, d, lens, dtype = case
     Q, K, V, Kd, Vd, mask = tree_inputs(n, h, hk, l, s, d, dtype, seed=l * 1000 + s + d, masks=masks)
