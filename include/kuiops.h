@@ -474,9 +474,7 @@ KUIOPS_API int kuiops_attn_mass(const kuiops_attn_mass_args* args, kuiops_stream
  * (n, h_kv, cap) int32, the token position of each slot; NULL: its slot; next_pos NULL: kv_lens.  A row with
  * kv_lens[g] <= budget keeps everything.  The inputs mass, pos and kv_lens are not written (and must not be the
  * outputs), so the call may be repeated.  1 <= budget <= cap, sinks + recent <= budget.  Elements of 1, 2 or 4 bytes.
- * workspace: kuiops_kv_evict_workspace_bytes(...) bytes, 4-byte aligned, no initial contents required.  No counterpart
- * in the reference. */
-KUIOPS_API size_t kuiops_kv_evict_workspace_bytes(uint32_t n, uint32_t h_kv, uint32_t cap, uint32_t budget);
+ * No counterpart in the reference. */
 typedef struct kuiops_kv_evict_args {
   void *K, *V;
   const float* mass;
@@ -485,9 +483,7 @@ typedef struct kuiops_kv_evict_args {
   float* mass_out;
   int32_t *pos_out, *src;
   int64_t* lens_out;
-  void* workspace;
   int64_t k_sn, k_sh, k_ss, v_sn, v_sh, v_ss;
-  uint64_t workspace_bytes;
   uint32_t elem_bytes, n, h_kv, cap, e, ev, lens_n, budget, sinks, recent;
 } kuiops_kv_evict_args;
 KUIOPS_API int kuiops_kv_evict(const kuiops_kv_evict_args* args, kuiops_stream_t stream);

@@ -97,7 +97,6 @@ SIGNATURES = {
     "kuiops_tree_accept": (c_int, [c_u32, c_u32, c_void_p, c_i64] + [c_void_p] * 7),
     "kuiops_kv_append": (c_int, [c_void_p, c_void_p]),
     "kuiops_attn_mass": (c_int, [c_void_p, c_void_p]),
-    "kuiops_kv_evict_workspace_bytes": (c_size_t, [c_u32] * 4),
     "kuiops_kv_evict": (c_int, [c_void_p, c_void_p]),
     "kuiops_add_i64": (c_int, [c_u64, c_void_p, c_i64, c_void_p]),
     "kuiops_topk_f32": (c_int, [c_u32, c_u32, c_u32, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -553,7 +552,7 @@ def sdpa(Q, K, V, *, bias=None, scale=None, is_causal=False, need_lse=True, out=
 _TREE_ARGS = struct.Struct("=30Qi7IfI")
 _APPEND_ARGS = struct.Struct("=24Q8I")
 _MASS_ARGS = struct.Struct("=13Qi7Iif")
-_EVICT_ARGS = struct.Struct("=18Q10I")
+_EVICT_ARGS = struct.Struct("=16Q10I")
 
 
 def _refuse(what):
@@ -792,15 +791,12 @@ def kv_evict(K, V, mass, kv_lens, budget, *, pos=None, next_pos=None, sinks=0, r
     pos_out = torch.empty((n, hkv, cap), dtype=torch.int32, device=mass.device) if pos is None else torch.empty_like(pos)
     src = pos_out.new_empty((n, hkv, budget))
     lens_out = torch.empty_like(kv_lens)
-    L = lib()
-    wsb = L.kuiops_kv_evict_workspace_bytes(n, hkv, cap, budget)
-    ws = pos_out.new_empty((wsb + 3) // 4)
     k0, k1, k2, _ = K.stride()
     v0, v1, v2, _ = V.stride()
-    _check(L.kuiops_kv_evict(_EVICT_ARGS.pack(
+    _check(lib().kuiops_kv_evict(_EVICT_ARGS.pack(
         K.data_ptr(), V.data_ptr(), mass.data_ptr(), 0 if pos is None else pos.data_ptr(), kv_lens.data_ptr(),
-        0 if next_pos is None else next_pos.data_ptr(), mass_out.data_ptr(), pos_out.data_ptr(), src.data_ptr(), lens_out.data_ptr(), ws.data_ptr(),
-        k0, k1, k2 if k2 > e else e, v0, v1, v2 if v2 > ev else ev, wsb,
+        0 if next_pos is None else next_pos.data_ptr(), mass_out.data_ptr(), pos_out.data_ptr(), src.data_ptr(), lens_out.data_ptr(),
+        k0, k1, k2 if k2 > e else e, v0, v1, v2 if v2 > ev else ev,
         K.element_size(), n, hkv, cap, e, ev, g, budget, sinks, recent), _stream()), "kv_evict")
     return lens_out, mass_out, pos_out, src
 

@@ -142,11 +142,9 @@ def test_contracts_of_the_c_entries():
     assert mass(dtype=9) == mass(s=0) == mass(Q=0) == mass(lse=0) == mass(kv_lens=P, lens_n=3) == mass(scale=float("nan")) == _ffi.EINVAL
     assert mass(e=2000, q_sl=2000, k_ss=2000) == _ffi.EUNSUPPORTED
     evict = c_call("kv_evict", dict(elem_bytes=2, n=4, h_kv=2, cap=100, e=128, ev=128, lens_n=2, budget=10, K=P, V=P, mass=P, mass_out=P + 64, pos_out=P,
-                                    src=P, kv_lens=P, lens_out=P + 8, workspace=P, workspace_bytes=1 << 30, k_ss=128, v_ss=128))
+                                    src=P, kv_lens=P, lens_out=P + 8, k_ss=128, v_ss=128))
     assert evict(elem_bytes=3) == evict(budget=0) == evict(budget=101) == evict(sinks=6, recent=5) == evict(lens_n=3) == _ffi.EINVAL
     assert evict(sinks=0xFFFFFFFF, recent=2) == evict(mass=0) == evict(mass_out=P) == evict(lens_out=P) == _ffi.EINVAL
-    short = L.kuiops_kv_evict_workspace_bytes(4, 2, 100, 10) - 1
-    assert evict(workspace=0) == evict(workspace_bytes=short) == evict(workspace=P + 2) == _ffi.EWORKSPACE
 
 
 # ------------------------------------------------------------------------------------------------
@@ -576,7 +574,7 @@ def check_evict(K, V, mass, lens, budget, *, pos=None, next_pos=None, sinks=0, r
 @pytest.mark.parametrize("lens,cap,budget,sinks,recent", [
     ([5], 5, 1, 0, 0), ([5], 5, 5, 2, 3), ([33], 40, 32, 0, 0), ([1, 0, -3], 40, 7, 0, 2), ([64, 1 << 40], 64, 20, 4, 8),
     ([1000, 1024, 1025], 1100, 500, 4, 100), ([2050, 31], 2100, 2049, 1, 1), ([5000], 5000, 100, 10, 90), ([4097, 4096], 4100, 3000, 0, 0),
-    ([33000], 33000, 16000, 4, 64),
+    ([33000], 33000, 16000, 4, 64), ([400000], 400000, 1000, 4, 64),       # keys kept in shared memory over a cluster, and too many for it
 ])
 def test_kv_evict(cuda, lens, cap, budget, sinks, recent):
     g = torch.Generator().manual_seed(cap + budget)
