@@ -15,6 +15,11 @@ collective"; tensor-parallel splits QKV / gate-up by output columns and O / down
 across ``tp`` ranks with one all-reduce after each row-split GEMM (two per layer): NCCL, or for
 decode-sized steps the fused form (``enable_fused_allreduce``) in which the GEMM epilogue stores
 its partial product into every rank's memory and the following RMSNorm sums the partials.
+
+Speculative steps and a bounded cache: ``verify`` scores a tree of drafted tokens in one pass over the cache, accepts
+the greedy path and commits it (every layer in one call); ``evict`` keeps the slots with the most accumulated attention
+weight.  From the first of these on a slot of the cache is no longer its token's position, so the state is per sequence
+and on the device (``kv_lens``, ``next_pos``), and decoding goes on with ``verify`` (a tree of one node is a plain step).
 """
 from dataclasses import dataclass
 
@@ -50,6 +55,31 @@ class DecoderConfig:
         per_layer = (self.d_model * (self.n_heads + 2 * self.n_kv_heads) * self.head_dim
                      + self.n_heads * self.head_dim * self.d_model + 3 * self.d_model * self.d_ff + 2 * self.d_model)
         return self.n_layers * per_layer + 2 * self.vocab * self.d_model + self.d_model
+
+
+class TreePlan:
+    """A tree of drafted tokens, the same for every sequence and step: ``parents[i]`` is the node above node i, -1 for the
+    root (node 0, the token that is certain); a node comes after its parent.  Holds what the kernels read: the parents,
+    the mask (a node sees itself and its ancestors) and the depths."""
+
+    def __init__(self, parents, device="cuda"):
+        parents = [int(p) for p in parents]
+        if not parents or parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i):
+            raise ValueError("a tree starts with its root (-1), and every other node comes after its parent")
+        n = len(parents)
+        mask = torch.zeros((n, n), dtype=torch.bool)
+        for i, p in enumerate(parents):
+            if i:
+                mask[i] = mask[p]
+            mask[i, i] = True
+        self.size, self.max_depth = n, int(mask.sum(1).max())
+        self.parents = torch.tensor(parents, dtype=torch.int64, device=device)
+        self.mask = mask.to(device)
+        self.depth = (mask.sum(1) - 1).to(device)
+
+    @staticmethod
+    def chain(n, device="cuda"):
+        return TreePlan(range(-1, n - 1), device)
 
 
 def shard_out_features(t, n_blocks_total, block, rank, size):
@@ -120,6 +150,7 @@ class Decoder:
             self.lm_head = shard_out_features(self.lm_head, cfg.vocab, 1, tp_rank, tp_size).clone()   # a copy: the slice would keep all rows alive
         self.vocab_lo = tp_rank * (cfg.vocab // tp_size)
         self.k_cache = self.v_cache = None
+        self.mass = self.kv_lens = None
         self.cap = 0
         self.length = 0
         self.exchange, self.exchange_rows = None, 0
@@ -150,11 +181,17 @@ class Decoder:
                         g.fill_(1.0)
 
     # ---- state ---------------------------------------------------------------------------
-    def alloc_cache(self, batch, capacity):
+    def alloc_cache(self, batch, capacity, track_mass=False, window=64):
+        """track_mass: accumulate the attention weight every cache slot receives, from the last `window` rows of the prompt
+        and from every verified step on (what ``evict`` goes by)."""
         shape = (self.cfg.n_layers, batch, self.hk, capacity, self.cfg.head_dim)
         self.k_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
         self.v_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
         self.cap, self.length, self.batch = capacity, 0, batch
+        self.kv_lens = self.next_pos = self.slot_pos = None
+        self.mass_window = int(window)
+        rows = (self.cfg.n_layers * batch, self.hk, capacity)
+        self.mass = torch.zeros(rows, device=self.device, dtype=torch.float32) if track_mass else None
 
     def enable_fused_allreduce(self, max_rows=128):
         """Tensor-parallel groups only: map every rank's receive area (kuillm_b200.peer) so that steps
@@ -230,7 +267,14 @@ class Decoder:
             else:
                 k4 = self.k_cache[li][:, :, :end]
                 v4 = self.v_cache[li][:, :, :end]
-            _ffi.sdpa(q4, k4, v4, is_causal=True, need_lse=False, out=o4, kv_lens=kv_lens)
+            observe = self.mass is not None and start == 0
+            lse = _ffi.sdpa(q4, k4, v4, is_causal=True, need_lse=observe, out=o4, kv_lens=kv_lens)[1]
+            if observe:
+                # the prompt's last rows vote for its slots, as a window of observation
+                w = min(seq, self.mass_window)
+                mass = self.mass[li * B:(li + 1) * B]
+                _ffi.attn_mass(q4[:, :, seq - w:], self.k_cache[li], lse[:, :, seq - w:], kv_lens=torch.full((B,), seq, dtype=torch.int64, device=self.device),
+                               is_causal=True, mass=mass, out=mass)
             if fold and (folded_resid or _ffi.gemm_residual_ssq(attn, L["wo"], resid, ssq_b)):
                 if folded_resid:
                     _ffi.gemm_residual_ssq(attn, L["wo"], resid, ssq_b)          # resid += attn Wo^T, squares -> ssq_b
@@ -371,7 +415,7 @@ class Decoder:
         B, S = ids.shape
         assert self.k_cache is not None and S <= self.cap and self.length == 0
         positions = torch.arange(S, device=self.device).repeat(B)
-        if self.tp_size > 1 and B % 2 == 0 and B * S >= self.overlap_min_rows and B * S > self.exchange_rows:
+        if self.tp_size > 1 and B % 2 == 0 and B * S >= self.overlap_min_rows and B * S > self.exchange_rows and self.mass is None:
             out = self._forward_tp_overlap(ids, positions, S)
         else:
             out = self._forward(ids, positions, S)
@@ -379,9 +423,110 @@ class Decoder:
 
     def decode_step(self, ids, local_logits=False):
         B = ids.shape[0]
+        assert self.kv_lens is None, "the cache is no longer position by slot: go on with verify (a tree of one node)"
         positions = torch.full((B,), self.length, device=self.device, dtype=torch.int64)
         out = self._forward(ids.reshape(B, 1), positions, 1)
         return out if local_logits else self._full_logits(out)
+
+    # ---- trees of drafted tokens, bounded cache --------------------------------------------------
+    def _start_ragged(self):
+        """The cache as `prefill` and `decode_step` left it, seen per sequence: slots in use, the next token's position, and each
+        slot's position."""
+        B = self.batch
+        self.kv_lens = torch.full((B,), self.length, dtype=torch.int64, device=self.device)
+        self.next_pos = self.kv_lens.clone()
+        self.slot_pos = torch.arange(self.cap, dtype=torch.int32, device=self.device).expand(self.cfg.n_layers * B, self.hk, self.cap).contiguous()
+
+    def verify(self, tokens, plan, return_logits=False):
+        """One step over a tree: tokens [B, plan.size], node 0 the token that is certain (the last one accepted), the others drafted
+        below it.  One pass scores every node, the greedy path through the tree is accepted and its keys and values go to the
+        cache.  Returns (path [B, size] of accepted nodes, then -1; counts [B]; next token [B]), and the logits [B, size,
+        vocab / tp] if asked.  The caller keeps room: counts are at most plan.max_depth, kv_lens + max_depth at most the capacity."""
+        cfg, B, l = self.cfg, tokens.shape[0], plan.size
+        if self.k_cache is None or B != self.batch or tokens.shape[1] != l:
+            raise ValueError("verify: tokens [batch, plan.size] on an allocated cache")
+        if self.kv_lens is None:
+            self._start_ragged()
+        hd, hq, hk, rows = cfg.head_dim, self.hq, self.hk, B * l
+        W = (hq + 2 * hk) * hd
+        positions = (self.next_pos[:, None] + plan.depth).reshape(-1)
+        x = _ffi.embedding(self.embed, tokens.reshape(-1))
+        # the layers' projections and log-sum-exps stay until the path is known: commit and mass take all layers at once
+        qkv_all = torch.empty((cfg.n_layers, rows, W), device=self.device, dtype=cfg.dtype)
+        lse_all = torch.empty((cfg.n_layers * B, hq, l), device=self.device, dtype=torch.float32) if self.mass is not None else None
+
+        def heads(t, n_heads, first):
+            n = t.numel() // (l * W)
+            return t.as_strided((n, n_heads, l, hd), (l * W, hd, W, 1), t.storage_offset() + first * hd)
+        resid = x
+        for li, L in enumerate(self.layers):
+            h = _ffi.rmsnorm(x, L["n1"], cfg.eps, residual=resid if li else None)
+            qkv = qkv_all[li]
+            if not (rows <= 128 and hd == 128 and _ffi.gemm_rope_qkv(h, L["wqkv"], hq, hk, hd, positions, cfg.rope_theta, out=qkv) is not None):
+                _ffi.gemm(h, L["wqkv"], trans_b=True, out=qkv)
+                _ffi.rope_qkv(qkv, hq, hk, hd, positions, cfg.rope_theta)
+            attn = torch.empty((rows, hq * hd), device=self.device, dtype=cfg.dtype)
+            o4 = attn.as_strided((B, hq, l, hd), (l * hq * hd, hd, hq * hd, 1))
+            lse = _ffi.sdpa_tree(heads(qkv, hq, 0), self.k_cache[li], self.v_cache[li], self.kv_lens, heads(qkv, hk, hq), heads(qkv, hk, hq + hk),
+                                 plan.mask, need_lse=lse_all is not None, out=o4)[1]
+            if lse_all is not None:
+                lse_all[li * B:(li + 1) * B].copy_(lse)
+            o = self._allreduce(_ffi.gemm(attn, L["wo"], trans_b=True))
+            h2 = _ffi.rmsnorm(o, L["n2"], cfg.eps, residual=resid)
+            x = self._allreduce(_ffi.gemm(_ffi.gemm_swiglu(h2, L["wgu"]), L["wd"], trans_b=True))
+        hf = _ffi.rmsnorm(x, self.norm_f, cfg.eps, residual=resid)
+        logits = _ffi.gemm(hf, self.lm_head, trans_b=True)
+        target = self.next_token(logits).reshape(B, l)
+        path, counts, nxt = _ffi.tree_accept(plan.parents, tokens, target)
+        K, V = (c.reshape(cfg.n_layers * B, hk, self.cap, hd) for c in (self.k_cache, self.v_cache))
+        lens = _ffi.kv_append(K, V, self.kv_lens, heads(qkv_all, hk, hq), heads(qkv_all, hk, hq + hk), path=path, counts=counts,
+                              pos=self.slot_pos, next_pos=self.next_pos, mass=self.mass)
+        if self.mass is not None:
+            # accepted node path[t] counts for the slots up to its own, the nodes left out for none
+            q_lens = torch.zeros((B, l + 1), dtype=torch.int64, device=self.device)
+            seen = self.kv_lens[:, None] + 1 + torch.arange(l, device=self.device)
+            q_lens.scatter_(1, torch.where(path >= 0, path, l), seen)
+            _ffi.attn_mass(heads(qkv_all, hq, 0), K, lse_all, kv_lens=lens, q_lens=q_lens[:, :l], mass=self.mass, out=self.mass)
+        self.kv_lens = lens
+        self.next_pos = self.next_pos + counts
+        return (path, counts, nxt) + ((logits.reshape(B, l, -1),) if return_logits else ())
+
+    def evict(self, budget, sinks=4, recent=64):
+        """Keep `budget` slots per sequence, layer and KV head: the first `sinks` and last `recent` positions, then those with the most
+        attention weight.  Sequences within the budget keep everything."""
+        if self.mass is None:
+            raise ValueError("evict goes by accumulated attention weight: alloc_cache(..., track_mass=True)")
+        if self.kv_lens is None:
+            self._start_ragged()
+        n = self.cfg.n_layers * self.batch
+        K, V = (c.reshape(n, self.hk, self.cap, self.cfg.head_dim) for c in (self.k_cache, self.v_cache))
+        self.kv_lens, self.mass, self.slot_pos, src = _ffi.kv_evict(K, V, self.mass, self.kv_lens, budget, pos=self.slot_pos, next_pos=self.next_pos,
+                                                                    sinks=sinks, recent=recent)
+        return src
+
+    def generate_tree(self, ids, new_tokens, plan, propose, budget=None, sinks=4, recent=64):
+        """Greedy decoding with drafts: propose(last [B], step) gives the drafted tokens [B, plan.size - 1] below each sequence's last
+        token.  With a budget the cache is evicted down to it whenever the next step might not fit the capacity.  Returns the
+        generated ids [B, new_tokens], the same as greedy decoding without drafts (up to ties within rounding)."""
+        last = self.next_token(self.prefill(ids, local_logits=True))
+        out = [[int(t)] for t in last.tolist()]
+        used, step = ids.shape[1], 0
+        while min(len(o) for o in out) < new_tokens:
+            if used + plan.max_depth > self.cap:
+                if budget is None:
+                    raise ValueError("generate_tree: the cache is full; give it a budget")
+                self.evict(budget, sinks, recent)
+                used = min(used, budget)
+                if used + plan.max_depth > self.cap:
+                    raise ValueError("generate_tree: a budget has to leave room for a step")
+            tokens = torch.cat([last[:, None], propose(last, step)], 1) if plan.size > 1 else last[:, None]
+            path, counts, nxt = self.verify(tokens.contiguous(), plan)
+            said = torch.where(path >= 0, tokens.gather(1, path.clamp(min=0)), path)
+            for o, row, c, t in zip(out, said.tolist(), counts.tolist(), nxt.tolist()):
+                o += row[1:c] + [t]
+            used += int(counts.max())
+            last, step = nxt, step + 1
+        return torch.tensor([o[:new_tokens] for o in out], dtype=torch.int64, device=self.device)
 
     # ---- captured decode step -----------------------------------------------------------------
     def _graph_step(self):
