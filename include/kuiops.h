@@ -383,8 +383,8 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
  *     out_i = softmax(scale * q_i K^T) V,   lse_i = natural log-sum-exp (fp32, (n, h, l), may be NULL).
  * Q is (n, h, l, e), the cache K / V (n, h_kv, s, e) / (n, h_kv, s, ev), DK / DV (n, h_kv, l, e) / (n, h_kv, l, ev),
  * out (n, h, l, ev); element strides for (batch, head, row), innermost dimension contiguous; Q, DK and DV may be
- * views of the packed projection rows kuiops_rope_qkv leaves.  mask is bytes, l x l per entry, mask_sn bytes
- * from one entry to the next (0: one mask for all).  A key that a row does not see takes no part in it, whatever its
+ * views of the packed projection rows kuiops_rope_qkv leaves.  mask is bytes, l x l per entry, with strides for (entry,
+ * row, key); mask_sn = 0: one mask for all.  A key that a row does not see takes no part in it, whatever its
  * rows hold (infinities, NaN); a row that sees no key gives 0 and -inf.  fp32 accumulation; 16-bit types round the
  * softmax weights to the element type before the product with V, as kuiops_sdpa does.
  * s may be 0 (K and V may then be NULL).  e <= 1024, ev <= 256 (KUIOPS_EUNSUPPORTED beyond),
@@ -400,7 +400,7 @@ typedef struct kuiops_sdpa_tree_args {
   float* lse;
   void* workspace;
   int64_t q_sn, q_sh, q_sl, k_sn, k_sh, k_ss, v_sn, v_sh, v_ss;
-  int64_t dk_sn, dk_sh, dk_sl, dv_sn, dv_sh, dv_sl, o_sn, o_sh, o_sl, mask_sn;
+  int64_t dk_sn, dk_sh, dk_sl, dv_sn, dv_sh, dv_sl, o_sn, o_sh, o_sl, mask_sn, mask_sl, mask_sk;
   uint64_t workspace_bytes;
   int32_t dtype;
   uint32_t n, h, h_kv, l, s, e, ev;

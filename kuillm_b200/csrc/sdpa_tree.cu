@@ -9,7 +9,7 @@
 
 namespace kuiops {
 
-static_assert(sizeof(kuiops_sdpa_tree_args) == 280, "callers pack the block without padding");
+static_assert(sizeof(kuiops_sdpa_tree_args) == 296, "callers pack the block without padding");
 
 constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeLn2 = 0.6931471805599453f;
@@ -101,7 +101,7 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
     for (int r = 0; r < R; ++r) {
       const uint32_t row = rb * R + r;
       bool v = inside && row < rows;
-      if (v && drafted) v = mk[size_t(row % p.l) * p.l + j] != 0;
+      if (v && drafted) v = mk[int64_t(row % p.l) * p.mask_sl + int64_t(j) * p.mask_sk] != 0;
       vis[r] = __ballot_sync(0xffffffffu, v);
       const float s2 = v ? sc[r] * qmul : -INFINITY;
       const float mn = fmaxf(m[r], warp_max(s2));
@@ -299,7 +299,7 @@ int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream) 
   const int64_t e = a.e, ev = a.ev;
   if (a.q_sl < e || a.dk_sl < e || a.dv_sl < ev || a.o_sl < ev) return KUIOPS_EINVAL;
   if (a.s > 0 && (a.k_ss < e || a.v_ss < ev)) return KUIOPS_EINVAL;
-  if (a.mask_sn != 0 && a.mask_sn < int64_t(a.l) * a.l) return KUIOPS_EINVAL;
+  if (a.mask_sn < 0 || a.mask_sl < 0 || a.mask_sk < 0) return KUIOPS_EINVAL;
   if (!(a.scale - a.scale == 0.f)) return KUIOPS_EINVAL;          // a finite number
   cudaStream_t st = as_stream(stream);
   const bool tc = sdpa_tree_tc_eligible(a);

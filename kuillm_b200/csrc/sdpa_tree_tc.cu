@@ -342,7 +342,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     uint32_t g = 0, n_seg = 0;
     for (; seg.next(p); ++n_seg) {
       const uint32_t S = seg.skeys, cache_tiles = seg.of - (a.l + RTN - 1) / RTN;
-      const unsigned char* mrow = a.mask + int64_t(seg.sb) * a.mask_sn + size_t(row_valid ? li : 0) * a.l;
+      const unsigned char* mrow = a.mask + int64_t(seg.sb) * a.mask_sn + int64_t(row_valid ? li : 0) * a.mask_sl;
       int* odd = odd_flag + (n_seg & 1);
       float m_used = -INFINITY, l_run = 0.f;
       for (uint32_t j = 0; j < seg.count && ok; ++j, ++g) {
@@ -357,7 +357,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll 32
             for (int c = 0; c < NC; ++c) {
               const uint32_t k = copy * NC + c;
-              if (k < nv && mrow[key0 + k] != 0) vis |= 1ull << c;
+              if (k < nv && mrow[int64_t(key0 + k) * a.mask_sk] != 0) vis |= 1ull << c;
             }
           }
         } else if (nv < RTN) {
@@ -490,11 +490,11 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       float* recs = tree_tc_record(p.partials, a.ev, p.rows, p.row_tiles, range, seg.first == 0, rt, 0);
       // what was kept out of the product, for a row that sees it: columns c .. c + N - 1 of drafted position `pos`
       auto add_odd = [&](float* o, int N, uint32_t c, uint32_t pos) {
-        const unsigned char* mr = a.mask + int64_t(seg.sb) * a.mask_sn + size_t(pos) * a.l;
+        const unsigned char* mr = a.mask + int64_t(seg.sb) * a.mask_sn + int64_t(pos) * a.mask_sl;
         const uint32_t t_hi = seg.first + seg.count, d_lo = seg.first > cache_tiles ? (seg.first - cache_tiles) * RTN : 0;
         const uint32_t d_hi = t_hi > cache_tiles ? min((t_hi - cache_tiles) * RTN, a.l) : 0;
         for (uint32_t k = d_lo; k < d_hi; ++k) {
-          if (mr[k] == 0) continue;
+          if (mr[int64_t(k) * a.mask_sk] == 0) continue;
           const T* v = static_cast<const T*>(a.DV) + int64_t(seg.sb) * a.dv_sn + int64_t(seg.skvh) * a.dv_sh + int64_t(k) * a.dv_sl + c;
 #pragma unroll
           for (int x = 0; x < N; ++x) {

@@ -549,7 +549,7 @@ def sdpa(Q, K, V, *, bias=None, scale=None, is_causal=False, need_lse=True, out=
 # a KV cache across decode steps: trees of drafted tokens, bounded size
 # --------------------------------------------------------------------------------------------
 # the argument blocks of include/kuiops.h, field for field: pointers and strides, then counts
-_TREE_ARGS = struct.Struct("=30Qi7IfI")
+_TREE_ARGS = struct.Struct("=32Qi7IfI")
 _APPEND_ARGS = struct.Struct("=24Q8I")
 _MASS_ARGS = struct.Struct("=13Qi7Iif")
 _EVICT_ARGS = struct.Struct("=16Q10I")
@@ -637,8 +637,7 @@ def sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, *, scale=None, need_lse=True, out=
     V, v0, v1, v2 = _rows_last(V)
     Kd, d0, d1, d2 = _rows_last(Kd)
     Vd, e0, e1, e2 = _rows_last(Vd)
-    if not mask.is_contiguous():
-        mask = mask.contiguous()
+    mst = mask.stride()
     if out is None:
         out = Q.new_empty((n, h, l, ev))
     o0, o1, o2, _ = out.stride()
@@ -651,7 +650,7 @@ def sdpa_tree(Q, K, V, kv_lens, Kd, Vd, mask, *, scale=None, need_lse=True, out=
         Q.data_ptr(), K.data_ptr(), V.data_ptr(), Kd.data_ptr(), Vd.data_ptr(), mask.data_ptr(), 0 if kv_lens is None else kv_lens.data_ptr(),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr(),
         q0, q1, q2, k0, k1, k2, v0, v1, v2, d0, d1, d2, e0, e1, e2, o0, o1, o2 if o2 > ev else ev,
-        l * l if mask.dim() == 3 and mask.shape[0] > 1 else 0, wsb,
+        mst[0] if len(mst) == 3 and mask.shape[0] > 1 else 0, mst[-2], mst[-1], wsb,
         code, n, h, hkv, l, s, e, ev, e ** -0.5 if scale is None else scale, 0), _stream()), "sdpa_tree")
     return out, lse
 

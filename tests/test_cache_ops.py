@@ -127,7 +127,7 @@ def test_contracts_of_the_c_entries():
                                     o_sh=128, Q=P, K=P, V=P, DK=P, DV=P, mask=P, out=P, workspace=P,
                                     workspace_bytes=1 << 30, q_sl=128, k_ss=128, v_ss=128, dk_sl=128, dv_sl=128, o_sl=128, scale=0.1))
     assert tree(dtype=7) == tree(n=0) == tree(l=0) == tree(h=3) == tree(Q=0) == tree(K=0) == tree(mask=0) == tree(out=0) == _ffi.EINVAL
-    assert tree(k_ss=64) == tree(mask_sn=8) == tree(scale=float("nan")) == tree(scale=float("inf")) == _ffi.EINVAL
+    assert tree(k_ss=64) == tree(mask_sk=(1 << 64) - 1) == tree(scale=float("nan")) == tree(scale=float("inf")) == _ffi.EINVAL
     assert tree(e=2048) == tree(ev=512) == _ffi.EUNSUPPORTED and tree(l=5000) == _ffi.ELIMIT
     need = L.kuiops_sdpa_tree_workspace_bytes(_ffi.BF16, 1, 4, 2, 3, 100000, 128, 128)
     assert need > 0
@@ -287,6 +287,9 @@ def test_tree_views_strides_and_shared_mask(cuda, dtype, d):
     out, lse = _ffi.sdpa_tree(Q, K, V, None, Kd, Vd, mask, out=buf.transpose(1, 2))
     check_tree(Q, K, V, None, Kd, Vd, mask, dtype, out, lse)
     assert out.data_ptr() == buf.data_ptr()
+    for odd in (mask.t().contiguous().t(), torch.stack([mask] * 3, -1)[..., 1], mask.expand(n, l, l), mask[None]):       # the same mask, other strides
+        again, _ = _ffi.sdpa_tree(Q, K, V, None, Kd, Vd, odd)
+        assert torch.equal(again, out)
     full, _ = _ffi.sdpa_tree(Q, K, V, lens_t([1 << 40, s]), Kd, Vd, mask)
     none, nolse = _ffi.sdpa_tree(Q, K, V, lens_t([-5, 0]), Kd, Vd, mask, need_lse=False)
     assert torch.equal(full, out) and nolse is None
