@@ -12,7 +12,8 @@ namespace kuiops {
 static_assert(sizeof(kuiops_attn_mass_args) == 144, "callers pack the block without padding");
 
 constexpr float kMassLog2e = 1.4426950408889634f;
-constexpr int kMassRows = 16;                    // query rows staged at a time
+constexpr int kMassRows = 16;                    // query rows a group stages at a time
+constexpr uint32_t kMassRowGroups = 2;           // halves of a CTA that share its keys and take the staged rows in turn
 
 // Keys of entry b that row li counts for.
 __device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, uint32_t li, uint32_t S) {
@@ -21,19 +22,21 @@ __device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, ui
   return clamp_len((long long)li + 1 + (long long)S - (long long)p.l, S);
 }
 
-// SIMT form for every type, head dimension and stride: a thread owns a key, whose row it keeps in shared memory (rows
-// padded to an odd length: no bank conflicts), and dots it with sixteen query rows at a time, broadcast from shared
-// memory.  fp32 arithmetic throughout.
+// SIMT form for every type, head dimension and stride: a thread owns a key, whose row the CTA keeps in shared memory (padded to
+// an odd length: no bank conflicts), and dots it with sixteen query rows at a time, four features of them per broadcast load.
+// Two halves of the CTA take the blocks of sixteen rows in turn and are added at the end.  fp32 arithmetic throughout; bound by
+// shared-memory loads (20 for 64 multiply-adds).
 template <typename T>
 __global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
   extern __shared__ __align__(16) float sm[];
-  const uint32_t KT = blockDim.x, ep = p.e | 1u, e4 = (p.e + 3) & ~3u;
-  float* q_s = sm;                               // [kMassRows][e4]
+  const uint32_t KT = blockDim.x / kMassRowGroups, ep = ((p.e + 3) & ~3u) + 1, e4 = ep - 1;
+  const uint32_t half = threadIdx.x / KT, t = threadIdx.x - half * KT, warp = t >> 5, warps = KT >> 5, lane = threadIdx.x & 31;
+  float* q_s = sm + half * (kMassRows * (e4 + 2));              // [kMassRows][e4] of this half, then lse and limits
   float* lse_s = q_s + kMassRows * e4;
   uint32_t* lim_s = reinterpret_cast<uint32_t*>(lse_s + kMassRows);
-  float* k_s = reinterpret_cast<float*>(lim_s + kMassRows);     // [KT][ep]
+  float* k_s = sm + kMassRowGroups * (kMassRows * (e4 + 2));    // [KT][ep]
   const uint32_t kt = blockIdx.x % key_tiles, u = blockIdx.x / key_tiles, kvh = u % p.h_kv, b = u / p.h_kv;
-  const uint32_t G = p.h / p.h_kv, rows = G * p.l, key0 = kt * KT, j = key0 + threadIdx.x;
+  const uint32_t G = p.h / p.h_kv, rows = G * p.l, key0 = kt * KT, j = key0 + t;
   pdl_wait();
   pdl_trigger();
   const uint32_t S = p.kv_lens ? clamp_len(p.kv_lens[b % p.lens_n], p.s) : p.s;
@@ -41,38 +44,40 @@ __global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
   if (key0 < S) {
     const T* Kb = static_cast<const T*>(p.K) + int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh;
     const uint32_t nk = min(KT, S - key0);
-    for (uint32_t i = threadIdx.x; i < nk * p.e; i += KT)
-      k_s[(i / p.e) * ep + i % p.e] = ElemTraits<T>::to_f(Kb[int64_t(key0 + i / p.e) * p.k_ss + i % p.e]);
-    const float* krow = k_s + threadIdx.x * ep;
+    for (uint32_t r = threadIdx.x >> 5; r < nk; r += blockDim.x >> 5)
+      for (uint32_t c = lane; c < e4; c += 32) k_s[r * ep + c] = c < p.e ? ElemTraits<T>::to_f(Kb[int64_t(key0 + r) * p.k_ss + c]) : 0.f;
+    const float* krow = k_s + t * ep;
     const float qmul = p.scale * kMassLog2e;
-    for (uint32_t r0 = 0; r0 < rows; r0 += kMassRows) {
+    for (uint32_t r0 = half * kMassRows; r0 - half * kMassRows < rows; r0 += kMassRows * kMassRowGroups) {
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < kMassRows * e4; i += KT) {
-        const uint32_t row = r0 + i / e4, c = i % e4;
-        q_s[i] = row < rows && c < p.e ? ElemTraits<T>::to_f(static_cast<const T*>(p.Q)[int64_t(b) * p.q_sn +
-                     int64_t(kvh * G + row / p.l) * p.q_sh + int64_t(row % p.l) * p.q_sl + c]) : 0.f;
-      }
-      for (uint32_t i = threadIdx.x; i < kMassRows; i += KT) {
-        const uint32_t row = r0 + i;
-        float ls = INFINITY;
-        uint32_t lim = 0;
-        if (row < rows) {
-          ls = p.lse[(size_t(b) * p.h + kvh * G + row / p.l) * p.l + row % p.l];
-          // a row that saw nothing (-inf) or is not to be counted (+inf) has no weight to give
-          if (!isinf(ls)) lim = mass_limit(p, b, row % p.l, S);
+      for (uint32_t r = warp; r < kMassRows; r += warps) {
+        const uint32_t row = r0 + r, gh = row / p.l, li = row - gh * p.l;
+        const T* q = static_cast<const T*>(p.Q) + int64_t(b) * p.q_sn + int64_t(kvh * G + gh) * p.q_sh + int64_t(li) * p.q_sl;
+        for (uint32_t c = lane; c < e4; c += 32) q_s[r * e4 + c] = row < rows && c < p.e ? ElemTraits<T>::to_f(q[c]) : 0.f;
+        if (lane == 0) {
+          float ls = INFINITY;
+          uint32_t lim = 0;
+          if (row < rows) {
+            ls = p.lse[(size_t(b) * p.h + kvh * G + gh) * p.l + li];
+            // a row that saw nothing (-inf) or is not to be counted (+inf) has no weight to give
+            if (!isinf(ls)) lim = mass_limit(p, b, li, S);
+          }
+          lse_s[r] = ls * kMassLog2e;
+          lim_s[r] = lim;
         }
-        lse_s[i] = ls * kMassLog2e;
-        lim_s[i] = lim;
       }
       __syncthreads();
       if (j < S) {
         float sc[kMassRows];
 #pragma unroll
         for (int r = 0; r < kMassRows; ++r) sc[r] = 0.f;
-        for (uint32_t c = 0; c < p.e; ++c) {
-          const float kf = krow[c];
+        for (uint32_t c = 0; c < e4; c += 4) {
+          const float k0 = krow[c], k1 = krow[c + 1], k2 = krow[c + 2], k3 = krow[c + 3];
 #pragma unroll
-          for (int r = 0; r < kMassRows; ++r) sc[r] = fmaf(q_s[r * e4 + c], kf, sc[r]);
+          for (int r = 0; r < kMassRows; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(q_s + r * e4 + c);
+            sc[r] = fmaf(q.w, k3, fmaf(q.z, k2, fmaf(q.y, k1, fmaf(q.x, k0, sc[r]))));
+          }
         }
         float part = 0.f;
 #pragma unroll
@@ -82,23 +87,26 @@ __global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
       }
     }
   }
-  if (j < p.s) {
+  __syncthreads();
+  if (half == 1) sm[t] = total;                                  // the staged rows are done with
+  __syncthreads();
+  if (half == 0 && j < p.s) {
     const size_t o = (size_t(b) * p.h_kv + kvh) * p.s + j;
-    p.out[o] = (p.mass ? p.mass[o] : 0.f) + total;
+    p.out[o] = (p.mass ? p.mass[o] : 0.f) + (total + sm[t]);
   }
 }
 
 template <typename T>
 static int mass_simt_launch(const MassArgs& a, cudaStream_t st) {
   // a CTA's key rows have to fit shared memory: 128 keys of up to 256 features, 32 of up to 1024
-  const uint32_t KT = a.e <= 256 ? 128 : 32, tiles = (a.s + KT - 1) / KT;
-  const size_t smem = (size_t(kMassRows) * (((a.e + 3) & ~3u) + 2) + size_t(KT) * (a.e | 1u)) * sizeof(float);
+  const uint32_t KT = a.e <= 256 ? 128 : 32, tiles = (a.s + KT - 1) / KT, e4 = (a.e + 3) & ~3u;
+  const size_t smem = (size_t(kMassRowGroups) * kMassRows * (e4 + 2) + size_t(KT) * (e4 + 1)) * sizeof(float);
   auto kern = attn_mass_simt_kernel<T>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
     return KUIOPS_ELAUNCH;
   const uint64_t grid = uint64_t(a.n) * a.h_kv * tiles;
   if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
-  return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT), smem, st, a, tiles);
+  return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT * kMassRowGroups), smem, st, a, tiles);
 }
 
 int attn_mass_simt(const MassArgs& a, cudaStream_t st) {
