@@ -352,13 +352,14 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t nv = min(uint32_t(RTN), (drafted ? a.l : S) - key0);     // keys of the tile
         uint64_t vis = ~0ull;                                                   // this copy's columns the row sees
         if (drafted) {
+          // read without a branch, so that the loads are under way together: past the last key, it again
           vis = 0;
-          if (row_valid) {
+          const unsigned char* mk = mrow + int64_t(key0) * a.mask_sk;
 #pragma unroll 32
-            for (int c = 0; c < NC; ++c) {
-              const uint32_t k = copy * NC + c;
-              if (k < nv && mrow[int64_t(key0 + k) * a.mask_sk] != 0) vis |= 1ull << c;
-            }
+          for (int c = 0; c < NC; ++c) {
+            const uint32_t k = copy * NC + c;
+            const unsigned char seen = mk[int64_t(min(k, nv - 1)) * a.mask_sk];
+            vis |= uint64_t(row_valid && k < nv && seen != 0) << c;
           }
         } else if (nv < RTN) {
           const int left = int(nv) - int(copy * NC);
@@ -601,29 +602,32 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
 struct TreeMerge { FastDiv by_chunks, by_heads, by_rows, by_lt; };
 
-// Joins the records of the units that lie in several ranges, in range order.  A warp takes two rows of one unit, side by side: lane
-// c looks after the maximum and sum of record c, every lane after four columns of all records, the first four of which are on their
-// way before the maxima are known.  (Four rows one after the other took 16 us where this takes a few: it is all latency.)
-template <typename T>
-__global__ void __launch_bounds__(128)
+// Joins the records of the units that lie in several ranges.  WPR warps take two rows of one unit, side by side, warp w the records
+// w, w + WPR, ..; lane c looks after the maximum and sum of its c-th record, every lane after four columns of all of them, the first four
+// of which are on their way before the maxima are known.  The warps' results are added in warp order, so nothing depends on timing.
+// (Four rows one after the other took 16 us where this takes a few: it is all latency.)
+template <typename T, int WPR>
+__global__ void __launch_bounds__(256)
 sdpa_tree_tc_merge_kernel(const TreeTcParams p, const TreeMerge m) {
+  constexpr int N = 2, A = 4;                              // rows of a warp, records ahead
+  constexpr uint32_t PAIRS = 8 / WPR;                      // pairs of rows of a CTA
   const TreeArgs& a = p.a;
-  const uint32_t lane = threadIdx.x & 31, u = m.by_chunks.div(blockIdx.x), chunk = blockIdx.x - u * m.by_chunks.d;
-  const uint32_t b = m.by_heads.div(u), kvh = u - b * a.h_kv;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR;
+  const uint32_t u = m.by_chunks.div(blockIdx.x), chunk = blockIdx.x - u * m.by_chunks.d, b = m.by_heads.div(u), kvh = u - b * a.h_kv;
   // The key counts are complete before the attention kernel's CTAs let this one start (each waited for them first); only the
   // records have to be waited for.
   const TreePlaces pl = tree_places(a, b);
   const uint32_t per = max((pl.all * a.h_kv + p.ranges - 1) / p.ranges, p.min_places), tiles = tree_tiles(a, tree_keys(a, b));
   const uint32_t begin = pl.before * a.h_kv + kvh * (tiles + kTreeLead) + kTreeLead;
-  const uint32_t c0 = begin / per, more = (begin + tiles - 1) / per - c0;
+  const uint32_t c0 = begin / per, pieces = (begin + tiles - 1) / per - c0 + 1;
   pdl_wait();
   pdl_trigger();
-  if (more == 0) return;                                   // whole: written already
+  if (pieces == 1) return;                                 // whole: written already
   const uint32_t rl = tree_record_floats(a.ev), tail = rl - 4, col = lane * 4;       // ev <= 128
   const size_t begins = size_t(p.row_tiles) * p.rows * rl, step = 2 * begins;        // from kind 0 to kind 1, and to the next range
   const bool on = col < a.ev;
-  constexpr int N = 2, A = 4;                              // rows of a warp, records ahead
-  const uint32_t row0 = (chunk * 4 + (threadIdx.x >> 5)) * N, all_rows = p.rows * p.row_tiles;
+  const uint32_t row0 = (chunk * PAIRS + warp / WPR) * N, all_rows = p.rows * p.row_tiles;
+  const uint32_t mine = part < pieces ? (pieces - part + WPR - 1) / WPR : 0;         // records of this warp
   const float *x[N], *y[N];                                // the unit's first record, and the next ones', which are of kind 0
   uint32_t gh[N], li[N];
   float mm[N], den[N], acc[N][4];
@@ -639,11 +643,15 @@ sdpa_tree_tc_merge_kernel(const TreeTcParams p, const TreeMerge m) {
     mm[i] = -INFINITY;
     den[i] = acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   }
-  auto md_of = [&](int i, uint32_t c) {
-    return c <= more ? __ldcg(reinterpret_cast<const float2*>((c == 0 ? x[i] : y[i] + (c - 1) * step) + tail)) : make_float2(-INFINITY, 0.f);
+  auto record = [&](int i, uint32_t k) {                    // this warp's k-th
+    const uint32_t c = part + k * WPR;
+    return c == 0 ? x[i] : y[i] + (c - 1) * step;
   };
-  auto cols_of = [&](int i, uint32_t c) {
-    return on && c <= more ? __ldcg(reinterpret_cast<const float4*>((c == 0 ? x[i] : y[i] + (c - 1) * step) + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  auto md_of = [&](int i, uint32_t k) {
+    return k < mine ? __ldcg(reinterpret_cast<const float2*>(record(i, k) + tail)) : make_float2(-INFINITY, 0.f);
+  };
+  auto cols_of = [&](int i, uint32_t k) {
+    return on && k < mine ? __ldcg(reinterpret_cast<const float4*>(record(i, k) + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
   };
 #pragma unroll
   for (int i = 0; i < N; ++i) md[i] = md_of(i, lane);
@@ -651,7 +659,7 @@ sdpa_tree_tc_merge_kernel(const TreeTcParams p, const TreeMerge m) {
   for (int k = 0; k < A; ++k)
 #pragma unroll
     for (int i = 0; i < N; ++i) ahead[i][k] = cols_of(i, k);
-  for (uint32_t k0 = 0; k0 <= more; k0 += 32) {
+  for (uint32_t k0 = 0; k0 < mine; k0 += 32) {
     float f[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -665,7 +673,7 @@ sdpa_tree_tc_merge_kernel(const TreeTcParams p, const TreeMerge m) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] *= g;
     }
-    for (uint32_t k = 0; k < min(32u, more + 1 - k0); k += A) {
+    for (uint32_t k = 0; k < min(32u, mine - k0); k += A) {
 #pragma unroll
       for (int q = 0; q < A; ++q)
 #pragma unroll
@@ -676,6 +684,33 @@ sdpa_tree_tc_merge_kernel(const TreeTcParams p, const TreeMerge m) {
           acc[i][2] = fmaf(fk, v.z, acc[i][2]); acc[i][3] = fmaf(fk, v.w, acc[i][3]);
           ahead[i][q] = cols_of(i, k0 + k + q + A);
         }
+    }
+  }
+  if constexpr (WPR > 1) {
+    __shared__ float join_s[8][N][32 * 4 + 2];
+    float* mine_s = join_s[warp][0];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float* to = mine_s + i * (32 * 4 + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e * 32 + lane] = acc[i][e];
+      if (lane == 0) { to[128] = mm[i]; to[129] = den[i]; }
+    }
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float top = -INFINITY;
+      for (int w = 0; w < WPR; ++w) top = fmaxf(top, join_s[warp + w][i][128]);
+      den[i] = acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+      for (int w = 0; w < WPR; ++w) {
+        const float* from = join_s[warp + w][i];
+        const float f = from[128] == -INFINITY ? 1.f : fast_ex2(from[128] - top);
+        den[i] = fmaf(f, from[129], den[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(f, from[e * 32 + lane], acc[i][e]);
+      }
+      mm[i] = top;
     }
   }
 #pragma unroll
@@ -744,10 +779,14 @@ static int tree_tc_launch(const CUtensorMap* m, const TreeTcParams& p, cudaStrea
   }
   const int rc = launch_pdl(kern, dim3(p.ranges * p.row_tiles), dim3(kTreeThreads), smem, st, m[0], m[1], m[2], m[3], m[4], p);
   if (rc != KUIOPS_OK || p.ranges == 1) return rc;
-  const uint32_t chunks = (p.rows * p.row_tiles + 7) / 8;                   // n h l is below 2^31: checked with the shape
+  // A unit has about ranges / units pieces.  More than eight are shared by eight warps (one unit of 64 rows, 65000 keys: 60 us with one
+  // warp a pair of rows, 30 with eight); few are not worth meeting for.
+  const uint32_t units = p.a.n * p.a.h_kv, wpr = p.ranges > 8 * units ? 8 : 1, pairs = 8 / wpr;
+  const uint32_t chunks = (p.rows * p.row_tiles + 2 * pairs - 1) / (2 * pairs);      // n h l is below 2^31: checked with the shape
   TreeMerge mg;
   mg.by_chunks.set(chunks); mg.by_heads.set(p.a.h_kv); mg.by_rows.set(p.rows); mg.by_lt.set(p.lt);
-  return launch_pdl(sdpa_tree_tc_merge_kernel<T>, dim3(p.a.n * p.a.h_kv * chunks), dim3(128), 0, st, p, mg);
+  auto merge = wpr == 8 ? sdpa_tree_tc_merge_kernel<T, 8> : sdpa_tree_tc_merge_kernel<T, 1>;
+  return launch_pdl(merge, dim3(units * chunks), dim3(256), 0, st, p, mg);
 }
 
 template <typename T, int DD>
