@@ -312,6 +312,23 @@ def test_tree_views_strides_and_shared_mask(cuda, dtype, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("h,hk,l", [(8, 8, 3), (16, 4, 12), (32, 8, 27)])
+def test_tree_and_mass_many_launches_never_time_out(cuda, h, hk, l):
+    """Every wait in the pipelines ends by its event: thousands of launches of uneven lengths leave the error word at zero, and
+    the last result is the first one's."""
+    Q, K, V, Kd, Vd, mask = tree_inputs(8, h, hk, l, 1500, 128, "bf16", seed=h)
+    lens = [lens_t([(i * 331 + j * 97) % 1501 for i in range(8)]) for j in range(5)]
+    first = [_ffi.sdpa_tree(Q, K, V, x, Kd, Vd, mask) for x in lens]
+    ones = [_ffi.attn_mass(Q, K, f[1], kv_lens=x, is_causal=False) for f, x in zip(first, lens)]
+    for _ in range(600):
+        last = [_ffi.sdpa_tree(Q, K, V, x, Kd, Vd, mask) for x in lens]
+        mass = [_ffi.attn_mass(Q, K, f[1], kv_lens=x, is_causal=False) for f, x in zip(first, lens)]
+    assert _ffi.tc_error() == 0
+    for a, b, c, d in zip(first, last, ones, mass):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(c, d)
+
+
+@pytest.mark.gpu
 def test_tree_with_other_value_dim(cuda):
     for d, dv, dtype in ((128, 64, "bf16"), (64, 128, "f16"), (40, 8, "bf16"), (20, 50, "f32")):
         Q, K, V, Kd, Vd, mask = tree_inputs(1, 4, 2, 5, 140, d, dtype, seed=d, dv=dv)
