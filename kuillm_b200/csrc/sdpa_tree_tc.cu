@@ -52,7 +52,10 @@ struct TreeTcParams {
 // this many empty places ahead of each unit.
 constexpr uint32_t kTreeLead = 3;
 
-__device__ __forceinline__ uint32_t tree_keys(const TreeArgs& a, uint32_t b) { return a.kv_lens ? clamp_len(a.kv_lens[b], a.s) : a.s; }
+// (From L2: the joining kernel reads the counts before it waits for the kernel ahead of it.)
+__device__ __forceinline__ uint32_t tree_keys(const TreeArgs& a, uint32_t b) {
+  return a.kv_lens ? clamp_len(__ldcg(reinterpret_cast<const long long*>(a.kv_lens) + b), a.s) : a.s;
+}
 __device__ __forceinline__ uint32_t tree_tiles(const TreeArgs& a, uint32_t keys) { return (keys + RTN - 1) / RTN + (a.l + RTN - 1) / RTN; }
 // Places of a KV head in all entries and in those before `b` (fewer than 2^31 in all: checked on the host); the whole warp
 // takes part.

@@ -580,6 +580,14 @@ def _buffer(kind, device, nbytes):
     return workspace(kind, device, nbytes)
 
 
+def _status_word(device):
+    """Address of the device's status word; none while a stream is being captured and there is no word yet (one made now would
+    only be zeroed when the graph runs)."""
+    if _capturing() and ("status", device.index, _stream()) not in _scratch:
+        return 0
+    return _status(device).data_ptr()
+
+
 def _rows_last(t):
     """Strides of a 4-D tensor whose innermost dimension is contiguous and whose rows do not overlap (a copy of it otherwise)."""
     a, b, c, d = t.stride()
@@ -673,7 +681,7 @@ def tree_accept(parents, draft, target):
     path = torch.empty_like(draft)
     counts, nxt = draft.new_empty((2, n)).unbind(0)
     _check(lib().kuiops_tree_accept(n, l, parents.data_ptr(), l if parents.dim() == 2 and parents.shape[0] > 1 else 0, draft.data_ptr(),
-                                    target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status(draft.device).data_ptr(),
+                                    target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status_word(draft.device),
                                     _stream()), "tree_accept")
     return path, counts, nxt
 
@@ -717,7 +725,7 @@ def kv_append(K, V, kv_lens, Kn, Vn, *, path=None, counts=None, pos=None, next_p
     _check(lib().kuiops_kv_append(_APPEND_ARGS.pack(
         Kn.data_ptr(), Vn.data_ptr(), K.data_ptr(), V.data_ptr(), kv_lens.data_ptr(), 0 if path is None else path.data_ptr(),
         0 if counts is None else counts.data_ptr(), 0 if next_pos is None else next_pos.data_ptr(), 0 if pos is None else pos.data_ptr(),
-        0 if mass is None else mass.data_ptr(), lens_out.data_ptr(), _status(K.device).data_ptr(),
+        0 if mass is None else mass.data_ptr(), lens_out.data_ptr(), _status_word(K.device),
         d0, d1, d2, e0, e1, e2, k0, k1, k2 if k2 > e else e, v0, v1, v2 if v2 > ev else ev,
         K.element_size(), n, hkv, l, cap, e, ev, g), _stream()), "kv_append")
     return lens_out

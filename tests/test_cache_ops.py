@@ -485,12 +485,14 @@ MASS_CASES = [
     (1, 2, 1, 5, 90, 300, [88], "f32"),
     (1, 160, 1, 2, 70, 128, [65], "bf16"),
     (5, 4, 2, 3, 600, 128, [600, 3, 64, 500, 599], "bf16"),
+    (300, 2, 1, 2, 40, 64, [2 + i % 39 for i in range(300)], "bf16"),           # more key counts than the kernel keeps on chip
+    (3, 12, 3, 120, 400, 128, [400, 120, 333], "f16"),                           # few row tiles, many items
 ]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("case", MASS_CASES, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
+@pytest.mark.parametrize("case", MASS_CASES, ids=lambda c: "-".join(str(x) for x in c[:6] + c[7:] + (c[6][:3],)).replace(" ", ""))
 def test_attn_mass(cuda, case, causal):
     n, h, hk, l, s, d, lens, dtype = case
     g = torch.Generator().manual_seed(l * 100 + s)
@@ -594,7 +596,7 @@ def check_evict(K, V, mass, lens, budget, *, pos=None, next_pos=None, sinks=0, r
 @pytest.mark.parametrize("lens,cap,budget,sinks,recent", [
     ([5], 5, 1, 0, 0), ([5], 5, 5, 2, 3), ([33], 40, 32, 0, 0), ([1, 0, -3], 40, 7, 0, 2), ([64, 1 << 40], 64, 20, 4, 8),
     ([1000, 1024, 1025], 1100, 500, 4, 100), ([2050, 31], 2100, 2049, 1, 1), ([5000], 5000, 100, 10, 90), ([4097, 4096], 4100, 3000, 0, 0),
-    ([33000], 33000, 16000, 4, 64), ([400000], 400000, 1000, 4, 64),       # keys kept in shared memory over a cluster, and too many for it
+    ([33000], 33000, 16000, 4, 64), ([300000], 300000, 200000, 4, 64), ([400000], 400000, 1000, 4, 64),       # keys kept in shared memory over a cluster, and too many for it
 ])
 def test_kv_evict(cuda, lens, cap, budget, sinks, recent):
     g = torch.Generator().manual_seed(cap + budget)
@@ -684,6 +686,40 @@ def test_verified_steps_equal_token_by_token_decoding(cuda):
     order = src.long().sort(-1).values[..., None].expand(n, hk, budget, d)
     want, wl = _ffi.sdpa(Q[:, :, :1], before.gather(2, order), values.gather(2, order), is_causal=True)
     assert (after.float() - want.float()).abs().max() <= 4 * 2.0 ** -8 * V.float().abs().max() and (al - wl).abs().max() < 1e-4
+
+
+@pytest.mark.gpu
+def test_calls_on_a_side_stream_first_captured_and_without_launch_overlap(cuda):
+    """A first use inside a capture on a fresh stream, replayed on changed inputs; and the same calls with programmatic launches
+    off."""
+    n, h, hk, l, s, d = 2, 8, 2, 5, 900, 128
+    Q, K, V, Kd, Vd, mask = tree_inputs(n, h, hk, l, s, d, "bf16", seed=41)
+    par, draft, target = (t.cuda() for t in accept_inputs(n, l, True, 7))
+    lens = lens_t([700, 650])
+    side = torch.cuda.Stream()
+
+    def step():
+        out, lse = _ffi.sdpa_tree(Q, K, V, lens, Kd, Vd, mask)
+        path, counts, nxt = _ffi.tree_accept(par, draft, target)
+        new = _ffi.kv_append(K, V, lens, Kd, Vd, path=path, counts=counts)
+        return out, lse, path, counts, nxt, new, _ffi.attn_mass(Q, K, lse, kv_lens=lens, is_causal=False)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        got = step()
+    for k in range(3):
+        Q.copy_(torch.randn(Q.shape, generator=torch.Generator().manual_seed(k)))
+        lens.copy_(lens_t([700 - k, 650 - 64 * k]))
+        gr.replay()
+        torch.cuda.synchronize()
+        have = [t.clone() for t in got]
+        want = step()
+        old = _ffi.set_pdl(False)
+        plain = step()
+        _ffi.set_pdl(old)
+        for a, b, c in zip(have, want, plain):
+            assert torch.equal(a, b) and torch.equal(a, c)
+    del gr
 
 
 @pytest.mark.gpu
