@@ -374,7 +374,7 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
 /* A KV cache across decode steps: trees of drafted tokens, bounded size    */
 /* ======================================================================== */
 #define KUIOPS_TREE_MAX_ROWS 4096u
-/* Most entry points of this section take their arguments as one block: passing forty arguments through a foreign
+/* The entry points of this section take their arguments as one block: passing forty arguments through a foreign
  * function interface costs more than the work of a small call.  A block is read before the call returns. */
 
 /* Attention of l drafted tokens (a tree, or any set of candidate continuations) over a cache plus their own
@@ -417,9 +417,14 @@ KUIOPS_API int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream
  * then -1; counts[n] their number (at least 1); next[n] = target of the chosen node.  A parent that does not come before
  * its node stores 1 in *status (which may be NULL) and the node is not accepted.  l <= KUIOPS_TREE_MAX_ROWS.
  * No counterpart in the reference. */
-KUIOPS_API int kuiops_tree_accept(uint32_t n, uint32_t l, const int64_t* parents, int64_t parents_sn,
-                const int64_t* draft, const int64_t* target, int64_t* path, int64_t* counts, int64_t* next,
-                int32_t* status, kuiops_stream_t stream);
+typedef struct kuiops_tree_accept_args {
+  const int64_t *parents, *draft, *target;
+  int64_t *path, *counts, *next;
+  int32_t* status;
+  int64_t parents_sn;
+  uint32_t n, l;
+} kuiops_tree_accept_args;
+KUIOPS_API int kuiops_tree_accept(const kuiops_tree_accept_args* args, kuiops_stream_t stream);
 
 /* Commits rows of DK / DV (n, h_kv, l, e | ev) to the caches K / V (n, h_kv, cap, e | ev): for t < counts[g] (all l when
  * counts is NULL) row path[g, t] (row t when path is NULL) goes to slot kv_lens[g] + t, where entry b uses

@@ -4,6 +4,7 @@
 
 namespace kuiops {
 
+static_assert(sizeof(kuiops_tree_accept_args) == 72, "callers pack the block without padding");
 static_assert(sizeof(kuiops_kv_append_args) == 224, "callers pack the block without padding");
 
 constexpr int kAcceptThreads = 128;
@@ -105,13 +106,14 @@ using namespace kuiops;
 
 extern "C" {
 
-int kuiops_tree_accept(uint32_t n, uint32_t l, const int64_t* parents, int64_t parents_sn, const int64_t* draft, const int64_t* target,
-                       int64_t* path, int64_t* counts, int64_t* next, int32_t* status, kuiops_stream_t stream) {
-  if (n == 0 || l == 0 || !parents || !draft || !target || !path || !counts || !next) return KUIOPS_EINVAL;
-  if (parents_sn != 0 && parents_sn < int64_t(l)) return KUIOPS_EINVAL;
-  if (l > KUIOPS_TREE_MAX_ROWS || n >= (1u << 31)) return KUIOPS_ELIMIT;
-  return launch_pdl(tree_accept_kernel, dim3(n), dim3(kAcceptThreads), size_t(l) * 4, as_stream(stream), l, parents, parents_sn, draft,
-                    target, path, counts, next, status);
+int kuiops_tree_accept(const kuiops_tree_accept_args* args, kuiops_stream_t stream) {
+  if (!args) return KUIOPS_EINVAL;
+  const kuiops_tree_accept_args& a = *args;
+  if (a.n == 0 || a.l == 0 || !a.parents || !a.draft || !a.target || !a.path || !a.counts || !a.next) return KUIOPS_EINVAL;
+  if (a.parents_sn != 0 && a.parents_sn < int64_t(a.l)) return KUIOPS_EINVAL;
+  if (a.l > KUIOPS_TREE_MAX_ROWS || a.n >= (1u << 31)) return KUIOPS_ELIMIT;
+  return launch_pdl(tree_accept_kernel, dim3(a.n), dim3(kAcceptThreads), size_t(a.l) * 4, as_stream(stream), a.l, a.parents, a.parents_sn, a.draft,
+                    a.target, a.path, a.counts, a.next, a.status);
 }
 
 int kuiops_kv_append(const kuiops_kv_append_args* args, kuiops_stream_t stream) {

@@ -75,19 +75,26 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
       const T* krow = drafted ? Kd + int64_t(j) * p.dk_sl : Kb + int64_t(j) * p.k_ss;
       uint32_t c = 0;
       if ((reinterpret_cast<uintptr_t>(krow) & 15u) == 0) {
-        constexpr int N = Vec16<T>::N;
-        for (; c + N <= p.e; c += N) {
-          const Vec16<T> kv = ld16(krow + c);
+        constexpr int N = Vec16<T>::N, A = 4;          // four vectors of the row under way
+        auto dot = [&](const Vec16<T>& kv, uint32_t at) {
           float kf[N];
 #pragma unroll
           for (int x = 0; x < N; ++x) kf[x] = ElemTraits<T>::to_f(kv.v[x]);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            const float* q = q_s + r * e_pad + c;
+            const float* q = q_s + r * e_pad + at;
 #pragma unroll
             for (int x = 0; x < N; ++x) sc[r] = fmaf(q[x], kf[x], sc[r]);
           }
+        };
+        for (; c + A * N <= p.e; c += A * N) {
+          Vec16<T> kv[A];
+#pragma unroll
+          for (int x = 0; x < A; ++x) kv[x] = ld16(krow + c + x * N);
+#pragma unroll
+          for (int x = 0; x < A; ++x) dot(kv[x], c + x * N);
         }
+        for (; c + N <= p.e; c += N) dot(ld16(krow + c), c);
       }
       for (; c < p.e; ++c) {
         const float kf = ElemTraits<T>::to_f(krow[c]);
@@ -117,20 +124,37 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
     uint32_t any = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) any |= vis[r];
+    // eight rows of V under way at a time (a loop over one row after the other is a chain of memory latencies: 76 against 25 us for
+    // one row over 4000 keys)
     const uint32_t d0 = lane * DV;
-    while (any) {
-      const int jj = __ffs(any) - 1;
-      any &= any - 1;
-      const T* vrow = drafted ? Vd + int64_t(key0 + jj) * p.dv_sl : Vb + int64_t(key0 + jj) * p.v_ss;
-      float vf[DV];
+    constexpr int B = DV == 8 ? 4 : 8;
+    for (uint32_t j0 = 0; j0 < 32; j0 += B) {
+      if (((any >> j0) & ((1u << B) - 1u)) == 0) continue;
+      float vf[B][DV];
 #pragma unroll
-      for (int d = 0; d < DV; ++d) vf[d] = (d0 + d < p.ev) ? ElemTraits<T>::to_f(vrow[d0 + d]) : 0.f;
+      for (int x = 0; x < B; ++x) {
+        const uint32_t jj = j0 + x;
+        const T* vrow = (drafted ? Vd + int64_t(key0 + jj) * p.dv_sl : Vb + int64_t(key0 + jj) * p.v_ss) + d0;
+        const bool seen = (any >> jj) & 1u;              // rows that nobody sees are not read
+        if (seen && d0 + DV <= p.ev && (reinterpret_cast<uintptr_t>(vrow) & (sizeof(T) * DV - 1)) == 0) {
+          struct alignas(sizeof(T) * DV) Pack { T v[DV]; };
+          const Pack w = *reinterpret_cast<const Pack*>(vrow);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float pj = __shfl_sync(0xffffffffu, pr[r], jj);
-        if ((vis[r] >> jj) & 1u) {
+          for (int d = 0; d < DV; ++d) vf[x][d] = ElemTraits<T>::to_f(w.v[d]);
+        } else {
 #pragma unroll
-          for (int d = 0; d < DV; ++d) acc[r][d] = fmaf(pj, vf[d], acc[r][d]);
+          for (int d = 0; d < DV; ++d) vf[x][d] = seen && d0 + d < p.ev ? ElemTraits<T>::to_f(vrow[d]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < B; ++x) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float pj = __shfl_sync(0xffffffffu, pr[r], j0 + x);
+          if ((vis[r] >> (j0 + x)) & 1u) {
+#pragma unroll
+            for (int d = 0; d < DV; ++d) acc[r][d] = fmaf(pj, vf[x][d], acc[r][d]);
+          }
         }
       }
     }
@@ -232,12 +256,12 @@ static int simt_launch_t(const TreeArgs& a, float* partials, uint32_t splits, cu
   return few ? simt_launch<T, 4, 8>(a, partials, splits, st) : simt_launch<T, 8, 8>(a, partials, splits, st);
 }
 
-// Slices per (batch, KV head, row block): as many CTAs as two waves hold (a 128-thread CTA, four to an SM), with at
-// least sixteen 32-key tiles each, so that joining stays small beside the keys read.
+// Slices per (batch, KV head, row block): as many CTAs as two waves hold (a 128-thread CTA, four to an SM), with at least
+// four 32-key tiles each, one per warp.
 uint32_t sdpa_tree_simt_splits(const TreeArgs& a) {
   const uint32_t rows = a.h / a.h_kv * a.l, R = rows <= 4 ? 4 : 8;
   const uint64_t units = uint64_t(a.n) * a.h_kv * ((rows + R - 1) / R), want = 8ull * num_sms() / units;
-  const uint32_t cap = (a.s / 32 + (a.l + 31) / 32) / 16;
+  const uint32_t cap = (a.s / 32 + (a.l + 31) / 32) / 4;
   const uint64_t v = want < cap ? want : cap;
   return v < 1 ? 1u : (v > 64 ? 64u : uint32_t(v));
 }

@@ -94,7 +94,7 @@ SIGNATURES = {
                             [c_void_p, c_float, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_void_p]),
     "kuiops_sdpa_tree_workspace_bytes": (c_size_t, [c_int] + [c_u32] * 7),
     "kuiops_sdpa_tree": (c_int, [c_void_p, c_void_p]),
-    "kuiops_tree_accept": (c_int, [c_u32, c_u32, c_void_p, c_i64] + [c_void_p] * 7),
+    "kuiops_tree_accept": (c_int, [c_void_p, c_void_p]),
     "kuiops_kv_append": (c_int, [c_void_p, c_void_p]),
     "kuiops_attn_mass": (c_int, [c_void_p, c_void_p]),
     "kuiops_kv_evict": (c_int, [c_void_p, c_void_p]),
@@ -550,6 +550,7 @@ def sdpa(Q, K, V, *, bias=None, scale=None, is_causal=False, need_lse=True, out=
 # --------------------------------------------------------------------------------------------
 # the argument blocks of include/kuiops.h, field for field: pointers and strides, then counts
 _TREE_ARGS = struct.Struct("=32Qi7IfI")
+_ACCEPT_ARGS = struct.Struct("=8Q2I")
 _APPEND_ARGS = struct.Struct("=24Q8I")
 _MASS_ARGS = struct.Struct("=13Qi7Iif")
 _EVICT_ARGS = struct.Struct("=16Q10I")
@@ -583,9 +584,12 @@ def _buffer(kind, device, nbytes):
 def _status_word(device):
     """Address of the device's status word; none while a stream is being captured and there is no word yet (one made now would
     only be zeroed when the graph runs)."""
-    if _capturing() and ("status", device.index, _stream()) not in _scratch:
-        return 0
-    return _status(device).data_ptr()
+    word = _scratch.get(("status", device.index, _stream()))
+    if word is None:
+        if _capturing():
+            return 0
+        word = _status(device)
+    return word.data_ptr()
 
 
 def _rows_last(t):
@@ -672,17 +676,17 @@ def tree_accept(parents, draft, target):
     n, l = draft.shape
     if parents.shape not in ((l,), (1, l), (n, l)):
         _refuse("tree_accept: parents [l] or [n,l]")
-    parents, draft, target = (_dense(t, torch.int64, "tree_accept: tokens and parents") for t in (parents, draft, target))
+    what = "tree_accept: tokens and parents"
+    parents, draft, target = _dense(parents, torch.int64, what), _dense(draft, torch.int64, what), _dense(target, torch.int64, what)
     dev = draft.get_device()
     ctx = _elsewhere(dev, "tree_accept", parents, target)
     if ctx is not None:
         with ctx:
             return tree_accept(parents, draft, target)
-    path = torch.empty_like(draft)
-    counts, nxt = draft.new_empty((2, n)).unbind(0)
-    _check(lib().kuiops_tree_accept(n, l, parents.data_ptr(), l if parents.dim() == 2 and parents.shape[0] > 1 else 0, draft.data_ptr(),
-                                    target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status_word(draft.device),
-                                    _stream()), "tree_accept")
+    path, counts, nxt = torch.empty_like(draft), draft.new_empty(n), draft.new_empty(n)
+    _check(lib().kuiops_tree_accept(_ACCEPT_ARGS.pack(
+        parents.data_ptr(), draft.data_ptr(), target.data_ptr(), path.data_ptr(), counts.data_ptr(), nxt.data_ptr(), _status_word(draft.device),
+        l if parents.dim() == 2 and parents.shape[0] > 1 else 0, n, l), _stream()), "tree_accept")
     return path, counts, nxt
 
 

@@ -102,7 +102,7 @@ def block(name):
         kind = "q" if "*" in decl or "int64_t" in decl else ("f" if "float" in decl else "i" if re.search(r"\bint32_t", decl) else "I")
         names = re.sub(r"\b(const|void|float|u?int\d+_t)\b|\*", " ", decl)
         fields += [(x.strip(), "Q" if kind == "q" and "uint64" not in decl else kind.upper() if "uint64" in decl else kind) for x in names.split(",")]
-    packer = getattr(_ffi, {"sdpa_tree": "_TREE_ARGS", "kv_append": "_APPEND_ARGS", "attn_mass": "_MASS_ARGS", "kv_evict": "_EVICT_ARGS"}[name])
+    packer = getattr(_ffi, {"sdpa_tree": "_TREE_ARGS", "tree_accept": "_ACCEPT_ARGS", "kv_append": "_APPEND_ARGS", "attn_mass": "_MASS_ARGS", "kv_evict": "_EVICT_ARGS"}[name])
     fmt = packer.format if isinstance(packer.format, str) else packer.format.decode()
     assert struct.Struct("=" + "".join(k for _, k in fields)).size == packer.size == struct.calcsize("@" + fmt[1:])
     return [f for f, _ in fields], packer
@@ -121,7 +121,7 @@ def c_call(name, defaults):
 
 def test_contracts_of_the_c_entries():
     L = _ffi.lib()
-    for name in ("sdpa_tree", "kv_append", "attn_mass", "kv_evict"):
+    for name in ("sdpa_tree", "tree_accept", "kv_append", "attn_mass", "kv_evict"):
         assert getattr(L, "kuiops_" + name)(None, None) == _ffi.EINVAL
     tree = c_call("sdpa_tree", dict(dtype=_ffi.BF16, n=1, h=4, h_kv=2, l=3, s=10, e=128, ev=128, q_sn=8, q_sh=128, k_sn=8, k_sh=128, v_sn=8, v_sh=128, dk_sh=128, dv_sh=128,
                                     o_sh=128, Q=P, K=P, V=P, DK=P, DV=P, mask=P, out=P, workspace=P,
@@ -132,8 +132,8 @@ def test_contracts_of_the_c_entries():
     need = L.kuiops_sdpa_tree_workspace_bytes(_ffi.BF16, 1, 4, 2, 3, 100000, 128, 128)
     assert need > 0
     assert tree(s=100000, workspace=0) == tree(s=100000, workspace_bytes=16) == tree(s=100000, workspace=P + 4) == _ffi.EWORKSPACE
-    acc = lambda n=2, l=5, par=P, sn=0: L.kuiops_tree_accept(n, l, par, sn, P, P, P, P, P, None, None)        # noqa: E731
-    assert acc(n=0) == acc(l=0) == acc(par=None) == acc(sn=4) == _ffi.EINVAL and acc(l=5000) == _ffi.ELIMIT
+    acc = c_call("tree_accept", dict(n=2, l=5, parents=P, draft=P, target=P, path=P, counts=P, next=P))
+    assert acc(n=0) == acc(l=0) == acc(parents=0) == acc(next=0) == acc(parents_sn=4) == _ffi.EINVAL and acc(l=5000) == _ffi.ELIMIT
     app = c_call("kv_append", dict(elem_bytes=2, n=4, h_kv=2, l=3, cap=8, e=128, ev=128, lens_n=2, DK=P, DV=P, K=P, V=P, kv_lens=P,
                                    dk_sl=128, dv_sl=128, k_ss=128, v_ss=128))
     assert app(elem_bytes=8) == app(n=0) == app(cap=0) == app(kv_lens=0) == app(lens_n=3) == app(lens_n=0) == app(pos=P) == app(k_ss=64) == _ffi.EINVAL
@@ -573,13 +573,14 @@ def check_evict(K, V, mass, lens, budget, *, pos=None, next_pos=None, sinks=0, r
             torch.full((n, hk, budget), -1, dtype=torch.int32)]
     before = [t.clone() for t in (mass,) + ((pos,) if pos is not None else ())]
     m, p = mass.cpu().numpy(), (pos.cpu().numpy() if pos is not None else np.broadcast_to(np.arange(cap), (n, hk, cap)))
+    k0, v0 = want[0].clone(), want[1].clone()
     for b in range(n):
         length = min(max(lens[b % g], 0), cap)
         for i in range(hk):
-            src = O.kv_evict_map(m[b, i], p[b, i], length, next_pos[b % g] if next_pos else length, budget, sinks, recent)
-            for to, frm in enumerate(src):
-                want[0][b, i, to], want[1][b, i, to] = K[b, i, frm].cpu(), V[b, i, frm].cpu()
-                want[2][b, i, to], want[3][b, i, to], want[4][b, i, to] = float(m[b, i, frm]), int(p[b, i, frm]), frm
+            src = torch.tensor(O.kv_evict_map(m[b, i], p[b, i], length, next_pos[b % g] if next_pos else length, budget, sinks, recent), dtype=torch.long)
+            k = len(src)
+            want[0][b, i, :k], want[1][b, i, :k] = k0[b, i, src], v0[b, i, src]
+            want[2][b, i, :k], want[3][b, i, :k], want[4][b, i, :k] = torch.from_numpy(m[b, i][src.numpy()]), torch.from_numpy(p[b, i][src.numpy()]).int(), src.int()
     got = _ffi.kv_evict(K, V, mass, lens_t(lens), budget, pos=pos, next_pos=lens_t(next_pos) if next_pos else None, sinks=sinks, recent=recent)
     assert got[0].tolist() == [min(min(max(x, 0), cap), budget) for x in lens]
     assert torch.equal(got[3].cpu(), want[4]) and torch.equal(got[2].cpu(), want[3])
