@@ -23,7 +23,8 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
   extern __shared__ __align__(16) float sm[];
   constexpr int ACCW = DV * 32 + 2;
   float* q_s = sm;                                  // [R][e_pad]
-  float* mrg = sm + R * e_pad;                      // [4 warps][R][ACCW]
+  float* p_s = sm + R * e_pad + (threadIdx.x >> 5) * R * 32;      // this warp's weights, [R][32]
+  float* mrg = sm + R * e_pad + 4 * R * 32;         // [4 warps][R][ACCW]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t split = blockIdx.x % splits;
   uint32_t u = blockIdx.x / splits;
@@ -121,9 +122,13 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
       for (int d = 0; d < DV; ++d) acc[r][d] *= corr;
       pr[r] = pv;
     }
-    uint32_t any = 0;
+    uint32_t any = 0, all = ~0u;
 #pragma unroll
-    for (int r = 0; r < R; ++r) any |= vis[r];
+    for (int r = 0; r < R; ++r) { any |= vis[r]; all &= vis[r]; }
+    __syncwarp();                                   // the weights of the tile before have been read
+#pragma unroll
+    for (int r = 0; r < R; ++r) p_s[r * 32 + lane] = pr[r];
+    __syncwarp();
     // eight rows of V under way at a time (a loop over one row after the other is a chain of memory latencies: 76 against 25 us for
     // one row over 4000 keys)
     const uint32_t d0 = lane * DV;
@@ -146,14 +151,27 @@ sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32
           for (int d = 0; d < DV; ++d) vf[x][d] = seen && d0 + d < p.ev ? ElemTraits<T>::to_f(vrow[d]) : 0.f;
         }
       }
+      if (all == ~0u) {                             // every row sees every key of the tile
 #pragma unroll
-      for (int x = 0; x < B; ++x) {
+        for (int x = 0; x < B; x += 4) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float pj = __shfl_sync(0xffffffffu, pr[r], j0 + x);
-          if ((vis[r] >> (j0 + x)) & 1u) {
+          for (int r = 0; r < R; ++r) {
+            const float4 pj = *reinterpret_cast<const float4*>(p_s + r * 32 + j0 + x);
 #pragma unroll
-            for (int d = 0; d < DV; ++d) acc[r][d] = fmaf(pj, vf[x][d], acc[r][d]);
+            for (int d = 0; d < DV; ++d)
+              acc[r][d] = fmaf(pj.w, vf[x + 3][d], fmaf(pj.z, vf[x + 2][d], fmaf(pj.y, vf[x + 1][d], fmaf(pj.x, vf[x][d], acc[r][d]))));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float pj = p_s[r * 32 + j0 + x];
+            if ((vis[r] >> (j0 + x)) & 1u) {
+#pragma unroll
+              for (int d = 0; d < DV; ++d) acc[r][d] = fmaf(pj, vf[x][d], acc[r][d]);
+            }
           }
         }
       }
@@ -239,7 +257,7 @@ sdpa_tree_merge_kernel(const TreeArgs p, const float* partials, uint32_t splits)
 template <typename T, int R, int DV>
 static int simt_launch(const TreeArgs& a, float* partials, uint32_t splits, cudaStream_t st) {
   const uint32_t e_pad = (a.e + 3) & ~3u, rows = a.h / a.h_kv * a.l, row_blocks = (rows + R - 1) / R;
-  const size_t smem = (size_t(R) * e_pad + size_t(4) * R * (DV * 32 + 2)) * sizeof(float);
+  const size_t smem = (size_t(R) * e_pad + size_t(4) * R * 32 + size_t(4) * R * (DV * 32 + 2)) * sizeof(float);
   auto kern = sdpa_tree_simt_kernel<T, R, DV>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
     return KUIOPS_ELAUNCH;
