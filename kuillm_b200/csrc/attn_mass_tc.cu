@@ -38,7 +38,7 @@ template <int DD, int NQ> struct MassTile {
   static constexpr uint32_t kQRing = kStream ? 4 : kKRing;
   static constexpr uint32_t kRows = kStream ? 32 : NQ;    // columns of a warp
   static constexpr uint32_t kBars = 2 * (kKRing + 2 * kQRing + kMassS) + 2;
-  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + kMassLens * 4 + kQRing * (2 * NQ + 4) * 4 + (kStream ? 2 * 3 * 128 * 4 : 0);
+  static constexpr uint32_t kSmem = kKRing * kKBytes + kQRing * kQBytes + kBars * 8 + kMassLens * 4 + kQRing * (2 * NQ + 4) * 4 + (kStream ? 4 * 4 * 128 * 4 : 0);
   static_assert(kSmem <= 227 * 1024, "one CTA per SM");
 };
 
@@ -132,7 +132,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint32_t* lens_s = reinterpret_cast<uint32_t*>(bars + MT::kBars);
   constexpr uint32_t RS = 2 * NQ + 4;    // words of a stage: -lse (log2 domain), limits, the least limit of each 32 rows
   float* row_s = reinterpret_cast<float*>(lens_s + kMassLens);
-  float* part_s = row_s + QR * RS;       // [2][3][128] sums of the groups behind the first
+  float* part_s = row_s + QR * RS;       // [4][group][128] sums of the groups, for four items
   const MassArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -295,7 +295,9 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (!STREAM && (any ? tile++ : round) % kMassGroups != group) continue;
       const size_t o = (size_t(it.b) * a.h_kv + it.kvh) * a.s + j;
       float total = 0.f, old = 0.f;
-      if ((!STREAM || group == 0) && a.mass && j < a.s) old = a.mass[o];
+      // the group that writes the item: with row tiles the one whose turn it is among those, else the one the round falls to
+      const bool writes = !STREAM || (any ? n_item : round) % kMassGroups == group;
+      if (writes && a.mass && j < a.s) old = a.mass[o];
       uint32_t nq = STREAM ? tile : tile - 1;
       for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
         const uint32_t sb = nq % kMassS, qb = nq % QR;
@@ -346,16 +348,22 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
       if constexpr (STREAM) {
         if (any) {
-          // the other groups' sums come through shared memory, added in group order; two buffers and one meeting per item: a
-          // thread that is an item ahead writes the other buffer
+          // The groups' sums meet in shared memory, in group order.  Only the group whose turn it is waits for the others; they go
+          // on with the next item.  A buffer comes up again four items later, and before that every group has waited for all the
+          // others once, in an item that the reader of this one had to reach first.
           tile = nq;
-          float* part = part_s + (n_item++ & 1) * 384;
-          if (group > 0) part[(group - 1) * 128 + key] = total;
-          asm volatile("bar.sync 1, 512;" ::: "memory");
-          if (group == 0) total += part[key] + part[128 + key] + part[256 + key];
+          const uint32_t slot = n_item++ % kMassGroups;
+          float* part = part_s + slot * (kMassGroups * 128) + key;
+          part[group * 128] = total;
+          if (writes) {
+            asm volatile("bar.sync %0, 512;" ::"r"(1 + slot) : "memory");
+            total = (part[0] + part[128]) + (part[256] + part[384]);
+          } else {
+            asm volatile("bar.arrive %0, 512;" ::"r"(1 + slot) : "memory");
+          }
         }
       }
-      if ((!STREAM || group == 0) && j < a.s && (a.mass != a.out || j < it.len)) a.out[o] = old + (j < it.len ? total : 0.f);
+      if (writes && j < a.s && (a.mass != a.out || j < it.len)) a.out[o] = old + (j < it.len ? total : 0.f);
     }
   }
   tc::tc_fence_before();
