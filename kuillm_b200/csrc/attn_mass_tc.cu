@@ -142,7 +142,8 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc::mbar_init(&q_full[i], 1); tc::mbar_init(&q_empty[i], 1);
       tc::mbar_init(&r_full[i], kMassRowWarps<NQ>); tc::mbar_init(&r_empty[i], STREAM ? 4 * kMassGroups : 4);
     }
-    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], STREAM ? 4 * kMassGroups : 4); }
+    // scores: the product's completion, and the issuer's word that the rows' values are there
+    for (uint32_t i = 0; i < kMassS; ++i) { tc::mbar_init(&s_full[i], 2); tc::mbar_init(&s_empty[i], STREAM ? 4 * kMassGroups : 4); }
     tc::fence_barrier_init();
   }
   if (warp == 1) {
@@ -223,6 +224,9 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                            (hh | kk) ? 1u : 0u);
           tc::umma_commit(&q_empty[qb]);
           tc::umma_commit(&s_full[sb]);
+          // one wait of this thread in place of one of every weight warp
+          if (!mass_wait(&r_full[qb], (nq / QR) & 1)) { atomicCAS(p.err, 0u, 58u); ok = false; break; }
+          tc::mbar_arrive(&s_full[sb]);
         }
         tc::umma_commit(&k_empty[kb]);
         ++nk;
@@ -301,7 +305,7 @@ attn_mass_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       uint32_t nq = STREAM ? tile : tile - 1;
       for (uint32_t qt = it.qt0; qt < it.qt1; ++qt, ++nq) {
         const uint32_t sb = nq % kMassS, qb = nq % QR;
-        if (ok && !__all_sync(0xffffffffu, mass_wait(&r_full[qb], (nq / QR) & 1) && mass_wait(&s_full[sb], (nq / kMassS) & 1))) {
+        if (ok && !__all_sync(0xffffffffu, mass_wait(&s_full[sb], (nq / kMassS) & 1))) {
           atomicCAS(p.err, 0u, 56u);
           ok = false;
         }
