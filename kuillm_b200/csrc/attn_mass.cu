@@ -13,7 +13,7 @@ static_assert(sizeof(kuiops_attn_mass_args) == 144, "callers pack the block with
 
 constexpr float kMassLog2e = 1.4426950408889634f;
 constexpr int kMassRows = 16;                    // query rows a group stages at a time
-constexpr uint32_t kMassRowGroups = 2;           // halves of a CTA that share its keys and take the staged rows in turn
+constexpr int kMassAhead = 4;                    // rows of Q or K a warp has under way together
 
 // Keys of entry b that row li counts for.
 __device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, uint32_t li, uint32_t S) {
@@ -24,17 +24,18 @@ __device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, ui
 
 // SIMT form for every type, head dimension and stride: a thread owns a key, whose row the CTA keeps in shared memory (padded to
 // an odd length: no bank conflicts), and dots it with sixteen query rows at a time, four features of them per broadcast load.
-// Two halves of the CTA take the blocks of sixteen rows in turn and are added at the end.  fp32 arithmetic throughout; bound by
-// shared-memory loads (20 for 64 multiply-adds).
+// `groups` parts of the CTA take the blocks of sixteen rows in turn and are added, in order, at the
+// end.  fp32 arithmetic throughout; bound by shared-memory loads (20 for 64 multiply-adds).
 template <typename T>
-__global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
+__global__ void __launch_bounds__(256)
+attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles, uint32_t groups) {
   extern __shared__ __align__(16) float sm[];
-  const uint32_t KT = blockDim.x / kMassRowGroups, ep = ((p.e + 3) & ~3u) + 1, e4 = ep - 1;
-  const uint32_t half = threadIdx.x / KT, t = threadIdx.x - half * KT, warp = t >> 5, warps = KT >> 5, lane = threadIdx.x & 31;
-  float* q_s = sm + half * (kMassRows * (e4 + 2));              // [kMassRows][e4] of this half, then lse and limits
+  const uint32_t KT = blockDim.x / groups, ep = ((p.e + 3) & ~3u) + 1, e4 = ep - 1;
+  const uint32_t part = threadIdx.x / KT, t = threadIdx.x - part * KT, warp = t >> 5, warps = KT >> 5, lane = threadIdx.x & 31;
+  float* q_s = sm + part * (kMassRows * (e4 + 2));              // [kMassRows][e4] of this part, then lse and limits
   float* lse_s = q_s + kMassRows * e4;
   uint32_t* lim_s = reinterpret_cast<uint32_t*>(lse_s + kMassRows);
-  float* k_s = sm + kMassRowGroups * (kMassRows * (e4 + 2));    // [KT][ep]
+  float* k_s = sm + groups * (kMassRows * (e4 + 2));    // [KT][ep]
   const uint32_t kt = blockIdx.x % key_tiles, u = blockIdx.x / key_tiles, kvh = u % p.h_kv, b = u / p.h_kv;
   const uint32_t G = p.h / p.h_kv, rows = G * p.l, key0 = kt * KT, j = key0 + t;
   pdl_wait();
@@ -44,26 +45,45 @@ __global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
   if (key0 < S) {
     const T* Kb = static_cast<const T*>(p.K) + int64_t(b) * p.k_sn + int64_t(kvh) * p.k_sh;
     const uint32_t nk = min(KT, S - key0);
-    for (uint32_t r = threadIdx.x >> 5; r < nk; r += blockDim.x >> 5)
-      for (uint32_t c = lane; c < e4; c += 32) k_s[r * ep + c] = c < p.e ? ElemTraits<T>::to_f(Kb[int64_t(key0 + r) * p.k_ss + c]) : 0.f;
+    const uint32_t all = blockDim.x >> 5;
+    for (uint32_t r = threadIdx.x >> 5; r < nk; r += kMassAhead * all)      // loads of several rows under way together
+      for (uint32_t c = lane; c < e4; c += 32) {
+        float v[kMassAhead];
+#pragma unroll
+        for (int x = 0; x < kMassAhead; ++x)
+          v[x] = r + x * all < nk && c < p.e ? ElemTraits<T>::to_f(Kb[int64_t(key0 + r + x * all) * p.k_ss + c]) : 0.f;
+#pragma unroll
+        for (int x = 0; x < kMassAhead; ++x)
+          if (r + x * all < nk) k_s[(r + x * all) * ep + c] = v[x];
+      }
     const float* krow = k_s + t * ep;
     const float qmul = p.scale * kMassLog2e;
-    for (uint32_t r0 = half * kMassRows; r0 - half * kMassRows < rows; r0 += kMassRows * kMassRowGroups) {
+    for (uint32_t r0 = part * kMassRows; r0 - part * kMassRows < rows; r0 += kMassRows * groups) {
       __syncthreads();
-      for (uint32_t r = warp; r < kMassRows; r += warps) {
-        const uint32_t row = r0 + r, gh = row / p.l, li = row - gh * p.l;
-        const T* q = static_cast<const T*>(p.Q) + int64_t(b) * p.q_sn + int64_t(kvh * G + gh) * p.q_sh + int64_t(li) * p.q_sl;
-        for (uint32_t c = lane; c < e4; c += 32) q_s[r * e4 + c] = row < rows && c < p.e ? ElemTraits<T>::to_f(q[c]) : 0.f;
-        if (lane == 0) {
-          float ls = INFINITY;
-          uint32_t lim = 0;
-          if (row < rows) {
-            ls = p.lse[(size_t(b) * p.h + kvh * G + gh) * p.l + li];
-            // a row that saw nothing (-inf) or is not to be counted (+inf) has no weight to give
-            if (!isinf(ls)) lim = mass_limit(p, b, li, S);
-          }
-          lse_s[r] = ls * kMassLog2e;
-          lim_s[r] = lim;
+      // lanes 0 to 15 look up one row each; all lanes then copy the features of one row after the other
+      const uint32_t row = r0 + (lane & (kMassRows - 1)), gh = row / p.l, li = row - gh * p.l;
+      const int64_t off = int64_t(b) * p.q_sn + int64_t(kvh * G + gh) * p.q_sh + int64_t(li) * p.q_sl;
+      if (warp == 0 && lane < kMassRows) {
+        float ls = INFINITY;
+        uint32_t lim = 0;
+        if (row < rows) {
+          ls = p.lse[(size_t(b) * p.h + kvh * G + gh) * p.l + li];
+          // a row that saw nothing (-inf) or is not to be counted (+inf) has no weight to give
+          if (!isinf(ls)) lim = mass_limit(p, b, li, S);
+        }
+        lse_s[lane] = ls * kMassLog2e;
+        lim_s[lane] = lim;
+      }
+      for (uint32_t r = warp; r < kMassRows; r += kMassAhead * warps) {     // `warps` is 1 or 4: whole batches
+        const T* q[kMassAhead];
+#pragma unroll
+        for (int x = 0; x < kMassAhead; ++x) q[x] = static_cast<const T*>(p.Q) + __shfl_sync(0xffffffffu, off, r + x * warps);
+        for (uint32_t c = lane; c < e4; c += 32) {
+          float v[kMassAhead];
+#pragma unroll
+          for (int x = 0; x < kMassAhead; ++x) v[x] = r0 + r + x * warps < rows && c < p.e ? ElemTraits<T>::to_f(q[x][c]) : 0.f;
+#pragma unroll
+          for (int x = 0; x < kMassAhead; ++x) q_s[(r + x * warps) * e4 + c] = v[x];
         }
       }
       __syncthreads();
@@ -79,34 +99,39 @@ __global__ void attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles) {
             sc[r] = fmaf(q.w, k3, fmaf(q.z, k2, fmaf(q.y, k1, fmaf(q.x, k0, sc[r]))));
           }
         }
-        float part = 0.f;
+        float w = 0.f;
 #pragma unroll
         for (int r = 0; r < kMassRows; ++r)
-          if (j < lim_s[r]) part += exp2f(fmaf(sc[r], qmul, -lse_s[r]));
-        total += part;
+          if (j < lim_s[r]) w += exp2f(fmaf(sc[r], qmul, -lse_s[r]));
+        total += w;
       }
     }
   }
   __syncthreads();
-  if (half == 1) sm[t] = total;                                  // the staged rows are done with
+  if (part > 0) sm[threadIdx.x] = total;                         // the staged rows are done with
   __syncthreads();
-  if (half == 0 && j < p.s) {
+  if (part == 0 && j < p.s) {
+    for (uint32_t g = 1; g < groups; ++g) total += sm[g * KT + t];
     const size_t o = (size_t(b) * p.h_kv + kvh) * p.s + j;
-    p.out[o] = (p.mass ? p.mass[o] : 0.f) + (total + sm[t]);
+    p.out[o] = (p.mass ? p.mass[o] : 0.f) + total;
   }
 }
 
 template <typename T>
 static int mass_simt_launch(const MassArgs& a, cudaStream_t st) {
-  // a CTA's key rows have to fit shared memory: 128 keys of up to 256 features, 32 of up to 1024
-  const uint32_t KT = a.e <= 256 ? 128 : 32, tiles = (a.s + KT - 1) / KT, e4 = (a.e + 3) & ~3u;
-  const size_t smem = (size_t(kMassRowGroups) * kMassRows * (e4 + 2) + size_t(KT) * (e4 + 1)) * sizeof(float);
+  // 128 keys and two parts; 32 keys and eight parts where that leaves SMs without work and there are rows to share (512 fp32 rows
+  // of 64 features over 95 keys of six heads: 103 against 26 us).  Wider heads: 32 keys with as many parts as fit shared memory.
+  const uint32_t e4 = (a.e + 3) & ~3u;
+  const bool spread = a.h / a.h_kv * a.l > 32 && uint64_t(a.n) * a.h_kv * ((a.s + 127) / 128) < 4ull * num_sms();
+  const uint32_t KT = a.e <= 256 && !spread ? 128 : 32, groups = a.e <= 256 ? (spread ? 8 : 2) : (a.e <= 512 ? 4 : 1);
+  const uint32_t tiles = (a.s + KT - 1) / KT;
+  const size_t smem = (size_t(groups) * kMassRows * (e4 + 2) + size_t(KT) * (e4 + 1)) * sizeof(float);
   auto kern = attn_mass_simt_kernel<T>;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
     return KUIOPS_ELAUNCH;
   const uint64_t grid = uint64_t(a.n) * a.h_kv * tiles;
   if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
-  return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT * kMassRowGroups), smem, st, a, tiles);
+  return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT * groups), smem, st, a, tiles, groups);
 }
 
 int attn_mass_simt(const MassArgs& a, cudaStream_t st) {

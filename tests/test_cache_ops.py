@@ -546,6 +546,25 @@ def test_attn_mass_row_limits_layers_views_and_scale(cuda, dtype, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,h,hk,l,s,d", [(3, 16, 2, 64, 98, 64), (1, 8, 8, 33, 397, 128), (1, 2, 1, 40, 70, 256), (1, 2, 2, 7, 45, 300),
+                                          (2, 4, 2, 9, 33, 512), (1, 2, 1, 20, 40, 513), (1, 2, 1, 35, 65, 1000), (1, 1, 1, 1, 2, 1024),
+                                          (1, 4, 2, 16, 300, 250), (150, 4, 4, 9, 600, 62), (2, 40, 1, 1, 130, 37)])
+def test_attn_mass_row_counts_and_wide_heads(cuda, dtype, n, h, hk, l, s, d):
+    """Few keys under many rows, many keys under few, heads up to the widest that is taken."""
+    g = torch.Generator().manual_seed(l + s)
+    Q, K = (torch.randn(*sh, generator=g).to(DT[dtype]).cuda() for sh in ((n, h, l, d), (n, hk, s, d)))
+    lens = [s - b % 5 for b in range(n)]
+    x = torch.einsum("nhld,nhsd->nhls", Q.double(), K.double().repeat_interleave(h // hk, 1)) * d ** -0.5
+    lim = [[i + 1 + lens[b] - l for i in range(l)] for b in range(n)]
+    seen = torch.arange(s).cuda() < torch.tensor(lim).cuda()[:, None, :, None]
+    lse = x.masked_fill(~seen, -float("inf")).logsumexp(-1).float()
+    mass = torch.rand(n, hk, s, generator=g).cuda()
+    out = _ffi.attn_mass(Q, K, lse, mass=mass, kv_lens=lens_t(lens), is_causal=True)
+    check_mass(Q, K, lse, lens, lim, mass, out)
+
+
+@pytest.mark.gpu
 def test_attn_mass_spreads_nan_only_where_it_belongs(cuda):
     g = torch.Generator().manual_seed(8)
     Q, K = torch.randn(1, 2, 4, 128, generator=g).bfloat16().cuda(), torch.randn(1, 2, 130, 128, generator=g).bfloat16().cuda()
