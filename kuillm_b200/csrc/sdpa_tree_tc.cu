@@ -6,6 +6,8 @@
 // A segment that is a whole unit writes its rows; the others leave records, which a second kernel joins.  (Joining them in the CTA
 // that finishes a unit last was slower, 87 against 69 us for 16 x 27 rows over 4096 keys: four warps cannot hide it.)  Rows beyond 128
 // per unit (G heads x lt drafted positions, one TMA box) go to further CTAs with the same range, which find the tiles in L2.
+// 32 / 8 heads of 128: 16 sequences x 27 rows over 2000 to 4001 keys 63 us (the stream alone 39 us, 5 TB/s); 2 x 64 rows over 65000 keys 170 us,
+// bound by the second row tile's passage through L2; 8 rows over 517 keys 12.5 us, launches and set-up.
 //
 // K and V tiles arrive through one in-order TMA ring (K0 V0 K1 V1 ...); S = Q K^T goes to TMEM (double buffered), the softmax
 // is online with one thread per row, P returns to TMEM over the scores it came from and is the A operand of O += P V.  Two
