@@ -389,7 +389,8 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
  * softmax weights to the element type before the product with V, as kuiops_sdpa does.
  * s may be 0 (K and V may then be NULL).  e <= 1024, ev <= 256 (KUIOPS_EUNSUPPORTED beyond),
  * l <= KUIOPS_TREE_MAX_ROWS.  workspace: kuiops_sdpa_tree_workspace_bytes(...) bytes, 16-byte aligned, no initial
- * contents required; calls that may overlap on the GPU need workspaces of their own.  No counterpart in the reference. */
+ * contents required; calls that may overlap on the GPU need workspaces of their own.  out and lse overlap none of the
+ * inputs.  No counterpart in the reference. */
 KUIOPS_API size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
                                    uint32_t l, uint32_t s, uint32_t e, uint32_t ev);
 typedef struct kuiops_sdpa_tree_args {
@@ -431,7 +432,8 @@ KUIOPS_API int kuiops_tree_accept(const kuiops_tree_accept_args* args, kuiops_st
  * g = b % lens_n, so that one call serves every layer of a model (n = layers * lens_n).  When given, pos (n, h_kv, cap)
  * receives next_pos[g] + t and mass (n, h_kv, cap) receives 0 at that slot.  lens_out[g] (may be NULL) =
  * kv_lens[g] + counts[g], at most cap; kv_lens itself is not written, and the call may be repeated.  Elements of
- * 1, 2 or 4 bytes.  A row or slot out of range is skipped and stores 1 in *status (which may be NULL).  No counterpart
+ * 1, 2 or 4 bytes.  Rows move in no order: DK and DV may lie in the cache's memory, but not in slots that the call
+ * writes.  A row or slot out of range is skipped and stores 1 in *status (which may be NULL).  No counterpart
  * in the reference (its caches grow by cat, kuiops/cat/wrapper_cat.cu.j2:28-34). */
 typedef struct kuiops_kv_append_args {
   const void *DK, *DV;
@@ -471,7 +473,8 @@ KUIOPS_API int kuiops_attn_mass(const kuiops_attn_mass_args* args, kuiops_stream
 
 /* Keeps `budget` of the kv_lens[g] slots of every (batch, KV head) row of a cache (g = b % lens_n): first the protected
  * ones (0 <= pos < sinks, or pos >= next_pos[g] - recent), then those with the largest mass (NaN above +inf, as
- * kuiops_topk_f32 orders them), equal ones by ascending slot.  The kept slots are not repacked: the i-th evicted slot
+ * kuiops_topk_f32 orders them), equal ones by ascending slot (protected ones are equal: where positions that repeat or
+ * lie ahead of next_pos protect more than budget, the lowest slots stay).  The kept slots are not repacked: the i-th evicted slot
  * below budget takes over the i-th kept slot at or above it, so attention over the first lens_out[g] =
  * min(kv_lens[g], budget) slots sees the kept keys, in another order.  K and V rows move in place; rows at or beyond
  * lens_out[g] stay as they were.  src (n, h_kv, budget) int32 = the slot each slot below budget came from (-1 beyond

@@ -413,7 +413,7 @@ class Decoder:
 
     def prefill(self, ids, local_logits=False):
         B, S = ids.shape
-        assert self.k_cache is not None and S <= self.cap and self.length == 0
+        assert self.k_cache is not None and S <= self.cap and self.length == 0 and self.kv_lens is None
         positions = torch.arange(S, device=self.device).repeat(B)
         if self.tp_size > 1 and B % 2 == 0 and B * S >= self.overlap_min_rows and B * S > self.exchange_rows and self.mass is None:
             out = self._forward_tp_overlap(ids, positions, S)
@@ -543,6 +543,7 @@ class Decoder:
 
     def capture_decode(self, batch):
         """Capture the decode step in a CUDA graph (launch-bound otherwise: ~290 kernels per token)."""
+        assert self.kv_lens is None, "the capture's warm-up writes the last slot, which may be in use after verify or evict"
         dev = self.device
         self._tok = torch.zeros(batch, dtype=torch.int64, device=dev)
         self._tok_out = torch.zeros(batch, dtype=torch.int64, device=dev)
@@ -572,6 +573,7 @@ class Decoder:
 
     def decode_graph(self, first_tok, steps, out=None):
         """Run `steps` captured decode steps starting from token `first_tok` at the current length."""
+        assert self.kv_lens is None, "the cache is no longer position by slot: go on with verify (a tree of one node)"
         B = first_tok.shape[0]
         if out is None:
             out = torch.empty((B, steps), dtype=torch.int64, device=self.device)

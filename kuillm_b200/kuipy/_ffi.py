@@ -694,7 +694,7 @@ def kv_append(K, V, kv_lens, Kn, Vn, *, path=None, counts=None, pos=None, next_p
     """Rows of Kn / Vn (n,h_kv,l,e|ev) into the caches K / V (n,h_kv,cap,e|ev), in place: row path[g,t] (t without a path)
     to slot kv_lens[g] + t for t < counts[g] (all l without counts).  kv_lens [g] int64 with n a multiple of g: entry b
     uses b % g, so the layers of a model go in one call.  pos int32 and mass fp32 (n,h_kv,cap) are set for the new slots
-    (next_pos[g] + t and 0).  Returns the new key counts [g]."""
+    (next_pos[g] + t and 0).  Kn and Vn are not slots that the call writes.  Returns the new key counts [g]."""
     if not (K.dim() == 4 and V.dim() == 4 and Kn.dim() == 4):
         _refuse("kv_append: 4-D tensors")
     n, hkv, cap, e = K.shape

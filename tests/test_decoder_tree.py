@@ -172,3 +172,29 @@ def test_generate_tree_equals_greedy_and_stays_within_its_cache(cuda):
     with pytest.raises(ValueError):
         dec.alloc_cache(2, 24)
         dec.generate_tree(ids, 60, plan, noise)
+
+
+@pytest.mark.gpu
+def test_paths_that_take_slots_for_positions_are_refused_after_a_tree_step(cuda):
+    dec = _decoder(64, seed=8)
+    ids = torch.randint(0, 1000, (1, 5), generator=torch.Generator().manual_seed(1)).cuda()
+    dec.alloc_cache(1, 16)
+    one = TreePlan.chain(1)
+    dec.verify(ids[:, :1], one)                                          # a cache may start with a tree step, without a prompt
+    for call in (lambda: dec.prefill(ids), lambda: dec.decode_step(ids[:, 0]), lambda: dec.capture_decode(1), lambda: dec.decode_graph(ids[:, 0], 1)):
+        with pytest.raises(AssertionError):
+            call()
+    dec.alloc_cache(1, 16)
+    dec.prefill(ids)
+    dec.decode_step(ids[:, 0])
+
+
+@pytest.mark.gpu
+def test_a_tree_step_without_a_prompt_equals_a_prompt(cuda):
+    dec = _decoder(64, seed=9)
+    ids = torch.randint(0, 1000, (2, 5), generator=torch.Generator().manual_seed(2)).cuda()
+    dec.alloc_cache(2, 16)
+    _, _, _, logits = dec.verify(ids, TreePlan.chain(5), return_logits=True)
+    with torch.no_grad():
+        want = _twin32(dec)(ids).logits
+    assert O.max_rel_err(to_np(logits), to_np(want)) <= 2e-2
