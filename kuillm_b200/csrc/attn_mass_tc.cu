@@ -88,7 +88,7 @@ __device__ __forceinline__ bool mass_item(const MassTcParams& p, const uint32_t*
   // that a causal mask's work falls with the item; with one the CTAs of a round read adjacent keys.
   const uint32_t id = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   if (round * gridDim.x >= p.items) return false;
-  if (id >= p.items) { it.qt0 = it.qt1 = 0; it.key0 = p.a.s; return true; }      // nothing in this round
+  if (id >= p.items) { it.qt0 = it.qt1 = 0; it.key0 = p.a.s; return true; }      // no item left for this turn
   const uint32_t hi = p.by_item.div(id), lo = id - hi * p.by_item.d;
   const uint32_t kt = p.q_tiles > 1 ? hi : lo, u = p.q_tiles > 1 ? lo : hi;
   it.b = p.by_heads.div(u);
