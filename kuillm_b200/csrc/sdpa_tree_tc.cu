@@ -19,7 +19,10 @@
 // slices.  The products cost the same (their M is 128 in any case).
 //
 // Masked keys take no part: cache rows behind the key count are zeroed in the V tile before the product, and so are the
-// drafted rows' elements that are not finite; those are added at the end to the rows that do see them.
+// drafted rows' elements that are not finite; those are added at the end to the rows that do see them.  The cache's own values
+// go into the product as they are, where an infinity among them meets the zeros of the other copies (and weights that round to
+// zero) and comes out as NaN: a segment whose O is not finite throughout reads its values again and puts such elements right
+// (odd_patch).  A finite cache pays one multiply-add per element of O for the question.
 #include "tree.cuh"
 #include "tc_ptx.cuh"
 #include <type_traits>
@@ -149,6 +152,13 @@ __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity) {
 // The same for a whole warp, which goes on or gives up as one.
 __device__ __forceinline__ bool tree_wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tree_wait(bar, parity)); }
 __device__ __forceinline__ void tree_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The same, and whether `v` is true in any of the four warps' threads.
+__device__ __forceinline__ bool tree_barrier_any(bool v) {
+  uint32_t any;
+  asm volatile("{.reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;}"
+               : "=r"(any) : "r"(uint32_t(v)) : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
@@ -165,6 +175,69 @@ __device__ __forceinline__ void tree_add2(float& a0, float& a1, float b0, float 
 }
 // Bits of a 16-bit element that are all set in infinities and NaN alone.
 template <typename T> __device__ __forceinline__ uint32_t exponent_bits() { return std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u; }
+
+// NaN where one of v[0 .. N - 1] is not finite, else 0.
+template <int N>
+__device__ __forceinline__ float odd_test(const float* v) {
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < N; ++c) t[c & 3] = fmaf(v[c], 0.f, t[c & 3]);
+  return (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+// A segment's values, and the row of the result (`out`, else its record `rec`) that a thread looks after (`row_on`).
+template <typename T> struct OddSegment {
+  const T *v, *dv;                      // the segment's cache rows, the drafted rows d_lo .. d_hi - 1
+  int64_t v_row, dv_row, mask_sk;
+  uint32_t keys, d_lo, d_hi, ev;
+  bool row_on;
+  const unsigned char* mask;
+  T* out;
+  float* rec;
+};
+// Elements of the result that came out not finite although the row's weights are: a sum with positive weights is what the visible
+// values that are not finite add up to, an infinity, or NaN where both signs or a NaN meet.  Elements whose values are all finite
+// stay.  The whole warp takes part, a lane with 16 bytes of a row of V.  Out of line: hardly ever called.
+template <typename T>
+__device__ __noinline__ void odd_patch(const OddSegment<T> g) {
+  const uint32_t lane = threadIdx.x & 31, piece = lane & 3, eb = exponent_bits<T>();
+  for (uint32_t c0 = 0; c0 < g.ev; c0 += 32) {
+    uint32_t pos = 0, neg = 0, nan = 0;                  // a bit per column
+    if (c0 + piece * 8 < g.ev) {
+      const T* at = g.v + c0 + piece * 8;
+      for (uint32_t k = lane >> 2; k < g.keys; k += 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(at + int64_t(k) * g.v_row);
+        const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const uint32_t y = (e[x / 2] >> (x % 2 * 16)) & 0xFFFFu, bit = 1u << (piece * 8 + x);
+          if ((y & eb) != eb) continue;
+          if (y & 0x7FFFu & ~eb) nan |= bit;
+          else if (y & 0x8000u) neg |= bit;
+          else pos |= bit;
+        }
+      }
+    }
+    pos = __reduce_or_sync(0xffffffffu, pos);
+    neg = __reduce_or_sync(0xffffffffu, neg);
+    nan = __reduce_or_sync(0xffffffffu, nan);
+    for (uint32_t c = 0; c < 32 && c0 + c < g.ev && g.row_on; ++c) {
+      if (isfinite(g.rec ? g.rec[c0 + c] : ElemTraits<T>::to_f(g.out[c0 + c]))) continue;
+      float y = 0.f;
+      if ((pos >> c) & 1u) y = INFINITY;
+      if ((neg >> c) & 1u) y -= INFINITY;
+      if ((nan >> c) & 1u) y = NAN;
+      for (uint32_t k = g.d_lo; k < g.d_hi; ++k) {
+        const float d = ElemTraits<T>::to_f(g.dv[int64_t(k) * g.dv_row + c0 + c]);
+        if (!isfinite(d) && g.mask[int64_t(k) * g.mask_sk] != 0) y += d;
+      }
+      if (y == 0.f) continue;
+      if (g.rec) g.rec[c0 + c] = y;
+      else g.out[c0 + c] = ElemTraits<T>::from_f(y);
+    }
+    __syncwarp();
+  }
+}
 
 // Six warps fill two of the SM's four register files twice and two once, so two CTAs need room for four warps in each: 128
 // registers a thread, which is what the bound for 256 threads says (for 192 it would be 168, and one CTA per SM).
@@ -517,6 +590,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         else if (a.lse)
           a.lse[(uint64_t(seg.sb) * a.h + seg.skvh * p.G + gh) * a.l + li] = den == 0.f ? -INFINITY : (mm + log2f(den)) * 0.6931471805599453f;
       }
+      float odd_o = 0.f;                                   // NaN once an element of O was not finite
       if constexpr (REP == 1) {
         // a thread holds its row: 64 bytes of it at a time
         T* orow = out_row(gh, li);
@@ -527,6 +601,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           tc::tmem_ld32(tmem_O + lane_addr + c0, ov);
           tc::tmem_ld_wait();
           if (!ok || !row_valid) continue;
+          odd_o += odd_test<32>(ov);
           if (bad) add_odd(ov, 32, c0, li);
           if (whole) {
 #pragma unroll
@@ -545,7 +620,6 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         __syncwarp();
         tc::tc_fence_before();
         if (lane == 0) tc::mbar_arrive(o_free);
-        tree_barrier();
       } else {
         // The copies meet in shared memory, 16 columns at a time; a thread then owns four columns of one row (two rows, where
         // there are up to 64) throughout.
@@ -566,6 +640,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           float ov[16];
           tc::tmem_ld16(tmem_O + lane_addr + c0, ov);
           tc::tmem_ld_wait();
+          odd_o += odd_test<16>(ov);
           tree_barrier();                                  // the columns before have been taken, at first: every sum read
           if (c0 == 0) ml[r128].y = inv;                   // the row's factor, for the threads that write its columns
 #pragma unroll
@@ -591,7 +666,21 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(o_free);
-        tree_barrier();
+      }
+      if (tree_barrier_any(odd_o != 0.f) && ok) {
+        OddSegment<T> sg;
+        const uint32_t t_hi = seg.first + seg.count, k_lo = seg.first * RTN, k_hi = min(min(t_hi, cache_tiles) * RTN, S);
+        sg.keys = k_hi > k_lo ? k_hi - k_lo : 0;
+        sg.v = static_cast<const T*>(a.V) + int64_t(seg.sb) * a.v_sn + int64_t(seg.skvh) * a.v_sh + int64_t(k_lo) * a.v_ss;
+        sg.dv = static_cast<const T*>(a.DV) + int64_t(seg.sb) * a.dv_sn + int64_t(seg.skvh) * a.dv_sh;
+        sg.d_lo = seg.first > cache_tiles ? (seg.first - cache_tiles) * RTN : 0;
+        sg.d_hi = t_hi > cache_tiles ? min((t_hi - cache_tiles) * RTN, a.l) : 0;
+        sg.v_row = a.v_ss; sg.dv_row = a.dv_sl; sg.ev = a.ev;
+        sg.mask = a.mask + int64_t(seg.sb) * a.mask_sn + int64_t(li) * a.mask_sl; sg.mask_sk = a.mask_sk;
+        sg.row_on = copy == 0 && row_valid && den == den;          // a NaN among the row's scores is the row's own
+        sg.out = out_row(gh, li);
+        sg.rec = whole ? nullptr : recs + size_t(r) * rl;
+        odd_patch<T>(sg);
       }
       if (tid == 0) *odd = 0;                              // this slot's next use is two segments away
     }

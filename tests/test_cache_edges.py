@@ -1,0 +1,52 @@
+"""Values, layouts, sizes and threads at which the operators on a KV cache can go wrong and that the tests of their ordinary
+range do not reach.  Error bounds as in test_cache_ops.py."""
+import numpy as np
+import pytest
+import torch
+
+from kuipy import _ffi
+from oracle import kuiops_oracle as O
+from test_cache_ops import check_tree, f64, lens_t, tree_inputs
+
+
+# ------------------------------------------------------------------------------------------------
+# tree attention: infinities and NaN in visible values of the cache
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,h,hk,l,s,d,lens,dtype,scale", [
+    (2, 4, 2, 2, 200, 128, [200, 67], "bf16", None),             # 4 rows per KV head
+    (1, 8, 2, 8, 130, 128, [129], "f16", None),                  # 32
+    (2, 8, 2, 9, 130, 128, [130, 64], "bf16", None),             # 36
+    (1, 8, 2, 16, 90, 64, [80], "f16", None),                    # 64
+    (1, 8, 2, 17, 129, 128, [128], "bf16", None),                # 68
+    (1, 8, 2, 32, 100, 64, [97], "f16", None),                   # 128
+    (1, 4, 1, 70, 90, 128, [77], "bf16", None),                  # 280: three tiles of rows
+    (1, 8, 2, 5, 5000, 128, [4999], "f16", None),                # keys split over CTAs, joined from records
+    (1, 8, 2, 24, 5000, 128, [4999], "bf16", None),
+    (40, 16, 8, 3, 200, 128, [71 + (i * 29) % 130 for i in range(40)], "bf16", None),      # CTAs that walk several units
+    (2, 6, 3, 5, 77, 80, [70, 77], "f16", None),                 # head dims that are no multiple of 64
+    (1, 4, 2, 6, 130, 40, [127], "bf16", None),
+    (1, 8, 2, 32, 300, 128, [300], "f16", 0.5),                  # weights below fp16's least, whose values still count
+    (1, 4, 2, 2, 300, 128, [300], "f16", 0.5),
+    (1, 2, 2, 4, 99, 33, [90], "bf16", None),                    # SIMT kernel
+    (1, 8, 2, 9, 1500, 64, [1400], "f32", None),
+])
+def test_tree_visible_values_that_are_not_finite(cuda, n, h, hk, l, s, d, lens, dtype, scale):
+    """A cache value that overflowed reaches every row that sees it as in a sum with positive weights: an infinity, or NaN
+    where both signs or a NaN meet; the other columns and the other heads stay as they are."""
+    Q, K, V, Kd, Vd, mask = tree_inputs(n, h, hk, l, s, d, dtype, seed=l + s)
+    inf, nan = float("inf"), float("nan")
+    for b in {0, n - 1}:
+        end = lens[b]
+        V[b, 0, 0, 0], V[b, 0, end - 1, 1] = inf, -inf
+        V[b, 0, 3, 2], V[b, 0, end // 2, 2] = inf, -inf
+        V[b, 0, 5, 3], V[b, 0, 6, 4], V[b, 0, 7, 4] = nan, inf, inf
+        V[b, hk - 1, end // 3, d - 1] = -inf
+        Vd[b, 0, 0, 0], Vd[b, 0, l // 2, 1] = -inf, -inf                        # meets the cache's +inf; adds to its -inf
+    out, lse = _ffi.sdpa_tree(Q, K, V, lens_t(lens), Kd, Vd, mask, scale=scale)
+    check_tree(Q, K, V, lens, Kd, Vd, mask, dtype, out, lse, scale=scale)
+    want = O.sdpa_tree(f64(Q), f64(K), f64(V), lens, f64(Kd), f64(Vd), mask.cpu().numpy(), scale)[0]
+    odd = np.isinf(want)
+    assert odd.any() and np.isnan(want).any() and np.array_equal(f64(out)[odd], want[odd])     # the sign too
+    again, _ = _ffi.sdpa_tree(Q, K, V, lens_t(lens), Kd, Vd, mask, scale=scale)
+    assert torch.equal(out.nan_to_num(5.0), again.nan_to_num(5.0)) and _ffi.tc_error() == 0
