@@ -301,7 +301,8 @@ KUIOPS_API int kuiops_bmm_f16 (uint32_t batch, uint32_t M, uint32_t K, uint32_t 
  * decode) run on the tcgen05 split-KV kernel, which spreads the keys of a
  * (batch, KV head) over several CTAs when there are few such pairs and then
  * needs kuiops_sdpa_workspace_bytes(...) of zero-initialised workspace (the query
- * returns 0 when no split is planned); everything else (bias, other head
+ * returns 0 when no split is planned; one buffer may serve calls of any shapes
+ * one after the other, the largest need deciding); everything else (bias, other head
  * dimensions, fp32) uses the generic SIMT kernel. */
 KUIOPS_API size_t kuiops_sdpa_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
                                    uint32_t l, uint32_t s, uint32_t e, uint32_t ev);
@@ -348,8 +349,8 @@ KUIOPS_API int kuiops_debug_sdpa_splits(int splits);
  * the library image (each GPU that loads the library holds one copy until the
  * process exits).  Inputs and outputs are still the caller's.  Arguments and
  * results are those of kuiops_sdpa_varlen (kv_lens may be NULL).
- *   - A problem whose scratch need exceeds the array is refused with
- *     KUIOPS_ELIMIT; nothing is launched.  The need is that of the kernel these
+ *   - A problem whose scratch need exceeds the array (its ticket words come on
+ *     top of the constant) is refused with KUIOPS_ELIMIT; nothing is launched.  The need is that of the kernel these
  *     arguments select (never more than kuiops_sdpa_workspace_bytes reports).
  *   - The array used is the copy on the GPU that holds Q, whichever device the
  *     calling thread has current; `stream` must belong to that GPU.  The first

@@ -28,6 +28,11 @@ struct SdpaRowsPlan {
 };
 
 SdpaRowsPlan sdpa_rows_plan(const SdpaArgs& a);
+// The ticket words of the split-KV kernels take the first kSdpaTicketBytes of their workspace, whatever the call: a buffer serves calls
+// of any shapes in turn, so no call's records may lie where a later call expects tickets that are zero.  More than kSdpaTickets
+// units are never split (they fill the GPU several times over).
+constexpr uint32_t kSdpaTickets = 1024;
+constexpr size_t kSdpaTicketBytes = kSdpaTickets * sizeof(int);
 size_t sdpa_rows_workspace_bytes(const SdpaArgs& a);
 size_t sdpa_rows_counter_bytes(const SdpaArgs& a);   // leading ticket words of that workspace
 int sdpa_rows(const SdpaArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st);

@@ -16,7 +16,8 @@ static int fill_args(SdpaArgs& a, int dtype, uint32_t n, uint32_t h, uint32_t h_
 // Scratch for kuiops_sdpa_noalloc: lives in the library image, one copy per GPU that loads it.
 // In host code the name below is only a handle; the device address comes from
 // cudaGetSymbolAddress, looked up once per device with that device current.
-static __device__ __align__(256) unsigned char g_sdpa_static_scratch[KUIOPS_SDPA_NOALLOC_SCRATCH_BYTES];
+constexpr size_t kSdpaStaticBytes = KUIOPS_SDPA_NOALLOC_SCRATCH_BYTES + kSdpaTicketBytes;     // records, and the tickets ahead of them
+static __device__ __align__(256) unsigned char g_sdpa_static_scratch[kSdpaStaticBytes];
 
 // Address of the array on device `dev`, which must be the current device.
 static int sdpa_static_scratch(int dev, void** out) {
@@ -143,7 +144,7 @@ int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32
   size_t need = 0, head = 0;
   if (which == kSdpaDecodeTc) { need = sdpa_decode_tc_workspace_bytes(a); head = sdpa_decode_tc_counter_bytes(a); }
   else if (which == kSdpaRows) { need = sdpa_rows_workspace_bytes(a); head = sdpa_rows_counter_bytes(a); }
-  if (need > size_t(KUIOPS_SDPA_NOALLOC_SCRATCH_BYTES)) return KUIOPS_ELIMIT;   // beyond the built-in scratch
+  if (need > kSdpaStaticBytes) return KUIOPS_ELIMIT;   // beyond the built-in scratch
   // The array to use is the copy on the GPU that holds Q, whichever device the calling thread
   // has current; that device is made current for the set-up, the clearing and the launch.
   cudaPointerAttributes attr = {};
@@ -164,8 +165,8 @@ int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32
   }
   switch (which) {
     case kSdpaFlash: return sdpa_flash(a, st);
-    case kSdpaDecodeTc: return sdpa_decode_tc(a, scratch, size_t(KUIOPS_SDPA_NOALLOC_SCRATCH_BYTES), st);
-    default: return sdpa_rows(a, scratch, size_t(KUIOPS_SDPA_NOALLOC_SCRATCH_BYTES), st);
+    case kSdpaDecodeTc: return sdpa_decode_tc(a, scratch, kSdpaStaticBytes, st);
+    default: return sdpa_rows(a, scratch, kSdpaStaticBytes, st);
   }
 }
 

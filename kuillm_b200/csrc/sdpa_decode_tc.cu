@@ -462,6 +462,7 @@ std::atomic<int> g_sdpa_splits_override{0};
 
 static uint32_t decode_tc_splits(const SdpaArgs& a) {
   const uint64_t units = uint64_t(a.n) * a.h_kv;
+  if (units > kSdpaTickets) return 1;
   const int forced = g_sdpa_splits_override.load(std::memory_order_relaxed);
   if (forced > 0) {
     const uint32_t tiles = (a.s + DBN - 1) / DBN;
@@ -482,7 +483,7 @@ size_t sdpa_decode_tc_workspace_bytes(const SdpaArgs& a) {
   if (splits == 1) return 0;
   const uint64_t units = uint64_t(a.n) * a.h_kv;
   const uint32_t rows = (a.h / a.h_kv) * a.l;
-  return ((units * 4 + 255) & ~size_t(255)) + size_t(units) * splits * rows * D_REC * sizeof(float);
+  return kSdpaTicketBytes + size_t(units) * splits * rows * D_REC * sizeof(float);
 }
 
 size_t sdpa_decode_tc_counter_bytes(const SdpaArgs& a) {
@@ -514,7 +515,7 @@ static int decode_tc_launch(const SdpaArgs& a, void* workspace, size_t workspace
       p.splits = 1;                 // no scratch: one CTA walks all keys of its (batch, KV head)
     } else {
       p.counters = static_cast<int*>(workspace);
-      p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((uint64_t(a.n) * a.h_kv * 4 + 255) & ~size_t(255)));
+      p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSdpaTicketBytes);
     }
   }
   CUtensorMap mq, mk, mv;

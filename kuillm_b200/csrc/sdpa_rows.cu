@@ -336,7 +336,7 @@ SdpaRowsPlan sdpa_rows_plan(const SdpaArgs& a) {
   pl.units = uint64_t(a.n) * pl.hgroups * pl.lblocks;
   pl.e_pad = (a.e + 7) & ~7u;
   pl.splits = 1;
-  if (pl.units < 2 * uint64_t(num_sms())) {
+  if (pl.units < 2 * uint64_t(num_sms()) && pl.units <= kSdpaTickets) {
     uint32_t want = uint32_t((4 * uint64_t(num_sms()) + pl.units - 1) / pl.units);
     uint32_t cap = a.s / 512;
     if (cap < 1) cap = 1;
@@ -352,8 +352,7 @@ SdpaRowsPlan sdpa_rows_plan(const SdpaArgs& a) {
 size_t sdpa_rows_workspace_bytes(const SdpaArgs& a) {
   SdpaRowsPlan pl = sdpa_rows_plan(a);
   if (pl.splits == 1) return 0;
-  const size_t counters = (size_t(pl.units) * 4 + 255) & ~size_t(255);
-  return counters + size_t(pl.units) * pl.splits * pl.r_pad * (pl.dv * 32 + 2) * sizeof(float);
+  return kSdpaTicketBytes + size_t(pl.units) * pl.splits * pl.r_pad * (pl.dv * 32 + 2) * sizeof(float);
 }
 
 size_t sdpa_rows_counter_bytes(const SdpaArgs& a) {
@@ -369,7 +368,7 @@ int sdpa_rows(const SdpaArgs& a, void* workspace, size_t workspace_bytes, cudaSt
       pl.splits = 1;        // no scratch: run unsplit rather than fail
     } else {
       pl.counters = static_cast<int*>(workspace);
-      pl.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((size_t(pl.units) * 4 + 255) & ~size_t(255)));
+      pl.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSdpaTicketBytes);
     }
   }
   const size_t esz = a.dtype == KUIOPS_F32 ? 4 : 2;
