@@ -118,18 +118,27 @@ attn_mass_simt_kernel(const MassArgs p, uint32_t key_tiles, uint32_t groups) {
   }
 }
 
+constexpr size_t mass_simt_smem(uint32_t e, uint32_t keys, uint32_t groups) {
+  const uint32_t e4 = (e + 3) & ~3u;
+  return (size_t(groups) * kMassRows * (e4 + 2) + size_t(keys) * (e4 + 1)) * sizeof(float);
+}
+constexpr size_t mass_most(size_t a, size_t b) { return a > b ? a : b; }
+// the widest head of each form below
+constexpr size_t kMassSimtSmem = mass_most(mass_most(mass_simt_smem(256, 128, 2), mass_simt_smem(256, 32, 8)),
+                                           mass_most(mass_simt_smem(512, 32, 4), mass_simt_smem(1024, 32, 1)));
+static_assert(kMassSimtSmem <= 227 * 1024, "shared memory of an SM");
+
 template <typename T>
 static int mass_simt_launch(const MassArgs& a, cudaStream_t st) {
   // 128 keys and two parts; 32 keys and eight parts where that leaves SMs without work and there are rows to share (512 fp32 rows
   // of 64 features over 95 keys of six heads: 103 against 26 us).  Wider heads: 32 keys with as many parts as fit shared memory.
-  const uint32_t e4 = (a.e + 3) & ~3u;
   const bool spread = a.h / a.h_kv * a.l > 32 && uint64_t(a.n) * a.h_kv * ((a.s + 127) / 128) < 4ull * num_sms();
   const uint32_t KT = a.e <= 256 && !spread ? 128 : 32, groups = a.e <= 256 ? (spread ? 8 : 2) : (a.e <= 512 ? 4 : 1);
   const uint32_t tiles = (a.s + KT - 1) / KT;
-  const size_t smem = (size_t(groups) * kMassRows * (e4 + 2) + size_t(KT) * (e4 + 1)) * sizeof(float);
+  const size_t smem = mass_simt_smem(a.e, KT, groups);
   auto kern = attn_mass_simt_kernel<T>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-    return KUIOPS_ELAUNCH;
+  static std::atomic<uint64_t> configured{0};
+  if (!raise_dynamic_smem(kern, kMassSimtSmem, configured)) return KUIOPS_ELAUNCH;
   const uint64_t grid = uint64_t(a.n) * a.h_kv * tiles;
   if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
   return launch_pdl(kern, dim3(unsigned(grid)), dim3(KT * groups), smem, st, a, tiles, groups);

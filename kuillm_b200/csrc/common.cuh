@@ -43,6 +43,19 @@ inline int check_launch() {
   return cudaPeekAtLastError() == cudaSuccess ? KUIOPS_OK : KUIOPS_ELAUNCH;
 }
 
+// Raises a kernel's limit of dynamic shared memory, once per device (`configured`: a bit each).  `bytes` is the most that any launch of
+// the kernel takes: a limit set to one call's need could fall below what another host thread is about to launch with.
+template <typename K>
+inline bool raise_dynamic_smem(K kern, size_t bytes, std::atomic<uint64_t>& configured) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (configured.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return false;
+  configured.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
 inline cudaStream_t as_stream(kuiops_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // ---- programmatic dependent launch -----------------------------------------------------------

@@ -294,14 +294,15 @@ sdpa_rows_kernel(const SdpaArgs p, const SdpaRowsPlan pl) {
   if (tid == 0) pl.counters[unit] = 0;
 }
 
+constexpr uint32_t kRowsMaxFeatures = 1024;       // of a query or key row
+
 template <typename T, int R, int DV>
 static int launch_rows(const SdpaArgs& a, const SdpaRowsPlan& pl, cudaStream_t st) {
   constexpr int ACCW = DV * 32 + 2;
   const size_t smem = (size_t(R) * pl.e_pad + size_t(5) * R * ACCW) * sizeof(float);
   auto kern = sdpa_rows_kernel<T, R, DV>;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-    return KUIOPS_ELAUNCH;
+  static std::atomic<uint64_t> configured{0};
+  if (!raise_dynamic_smem(kern, (size_t(R) * kRowsMaxFeatures + size_t(5) * R * ACCW) * sizeof(float), configured)) return KUIOPS_ELAUNCH;
   const uint64_t grid = uint64_t(pl.units) * pl.splits;
   if (grid >= (1ull << 31)) return KUIOPS_EUNSUPPORTED;
   kern<<<unsigned(grid), 128, smem, st>>>(a, pl);
@@ -361,7 +362,7 @@ size_t sdpa_rows_counter_bytes(const SdpaArgs& a) {
 }
 
 int sdpa_rows(const SdpaArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
-  if (a.ev > 256 || a.e > 1024) return KUIOPS_EUNSUPPORTED;
+  if (a.ev > 256 || a.e > kRowsMaxFeatures) return KUIOPS_EUNSUPPORTED;
   SdpaRowsPlan pl = sdpa_rows_plan(a);
   if (pl.splits > 1) {
     if (!workspace || workspace_bytes < sdpa_rows_workspace_bytes(a)) {

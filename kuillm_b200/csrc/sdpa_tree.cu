@@ -13,6 +13,7 @@ static_assert(sizeof(kuiops_sdpa_tree_args) == 296, "callers pack the block with
 
 constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeLn2 = 0.6931471805599453f;
+constexpr uint32_t kTreeMaxFeatures = 1024;      // of a query or key row
 
 // SIMT form: a CTA owns R query rows of one (batch, KV head) and a slice of the 32-key tiles (cache tiles first, then
 // the drafted ones).  Its four warps take tiles in turn; for the scores a lane owns a key and dots it with the R rows
@@ -258,10 +259,11 @@ sdpa_tree_merge_kernel(const TreeArgs p, const float* partials, uint32_t splits)
 template <typename T, int R, int DV>
 static int simt_launch(const TreeArgs& a, float* partials, uint32_t splits, cudaStream_t st) {
   const uint32_t e_pad = (a.e + 3) & ~3u, rows = a.h / a.h_kv * a.l, row_blocks = (rows + R - 1) / R;
-  const size_t smem = (size_t(R) * e_pad + size_t(4) * R * 32 + size_t(4) * R * (DV * 32 + 2)) * sizeof(float);
+  constexpr size_t fixed = (size_t(4) * R * 32 + size_t(4) * R * (DV * 32 + 2)) * sizeof(float);
+  const size_t smem = fixed + size_t(R) * e_pad * sizeof(float);
   auto kern = sdpa_tree_simt_kernel<T, R, DV>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-    return KUIOPS_ELAUNCH;
+  static std::atomic<uint64_t> configured{0};
+  if (!raise_dynamic_smem(kern, fixed + size_t(R) * kTreeMaxFeatures * sizeof(float), configured)) return KUIOPS_ELAUNCH;
   const uint64_t grid = uint64_t(a.n) * a.h_kv * row_blocks * splits;
   if (grid >= (1ull << 31)) return KUIOPS_ELIMIT;
   return launch_pdl(kern, dim3(unsigned(grid)), dim3(128), smem, st, a, partials, splits, row_blocks, e_pad);
@@ -310,7 +312,7 @@ using namespace kuiops;
 static int tree_shape(int dtype, uint32_t n, uint32_t h, uint32_t h_kv, uint32_t l, uint32_t s, uint32_t e, uint32_t ev) {
   if (dtype != KUIOPS_F32 && dtype != KUIOPS_BF16 && dtype != KUIOPS_F16) return KUIOPS_EINVAL;
   if (n == 0 || h == 0 || h_kv == 0 || l == 0 || e == 0 || ev == 0 || h % h_kv) return KUIOPS_EINVAL;
-  if (e > 1024 || ev > 256) return KUIOPS_EUNSUPPORTED;
+  if (e > kTreeMaxFeatures || ev > 256) return KUIOPS_EUNSUPPORTED;
   if (l > KUIOPS_TREE_MAX_ROWS || s > 0x7fffff00u || uint64_t(n) * h * l >= (1ull << 31)) return KUIOPS_ELIMIT;
   return KUIOPS_OK;
 }

@@ -50,3 +50,64 @@ def test_tree_visible_values_that_are_not_finite(cuda, n, h, hk, l, s, d, lens, 
     assert odd.any() and np.isnan(want).any() and np.array_equal(f64(out)[odd], want[odd])     # the sign too
     again, _ = _ffi.sdpa_tree(Q, K, V, lens_t(lens), Kd, Vd, mask, scale=scale)
     assert torch.equal(out.nan_to_num(5.0), again.nan_to_num(5.0)) and _ffi.tc_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------
+# host threads
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["tree", "mass", "sdpa"])
+def test_host_threads_with_different_head_sizes(cuda, op, monkeypatch):
+    """One kernel serves heads of all sizes and takes more than the default shared memory for wide ones: calls of two sizes from two
+    threads at once all launch, and give what they give alone."""
+    from threading import Barrier, Thread
+
+    def call(e, ev):
+        g = torch.Generator(device="cuda").manual_seed(e)
+        r = lambda *sh: torch.randn(*sh, generator=g, device="cuda")                             # noqa: E731
+        if op == "tree":
+            a = (r(1, 2, 8, e), r(1, 2, 32, e), r(1, 2, 32, ev), None, r(1, 2, 8, e), r(1, 2, 8, ev), torch.ones(8, 8, dtype=torch.bool, device="cuda"))
+            return lambda: _ffi.sdpa_tree(*a)
+        if op == "mass":
+            a = (r(1, 2, 8, e), r(1, 2, 32, e), torch.full((1, 2, 8), 3.0, device="cuda"))
+            return lambda: (_ffi.attn_mass(*a, is_causal=False),)
+        a = (r(1, 2, 16, e), r(1, 2, 32, e), r(1, 2, 32, ev))
+        return lambda: _ffi.sdpa(*a)
+
+    class Recorder:
+        """Makes the library's calls and keeps the arguments of each."""
+        def __getattr__(self, name):
+            def fn(*a):
+                self.last = (name, a)
+                return getattr(real, name)(*a)
+            return fn
+    real, rec = _ffi.lib(), Recorder()
+    monkeypatch.setattr(_ffi, "lib", lambda: rec)
+    made = []                                            # per thread: result, function and arguments, and what keeps them alive
+    for e in (1024, 420, 1024, 420):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            fn = call(e, 256)
+            made.append((fn(), rec.last, fn, stream))
+    monkeypatch.undo()
+    torch.cuda.synchronize()
+    alone = [res[0].clone() for res, *_ in made]
+    for res, *_ in made:
+        res[0].fill_(7.0)
+    torch.cuda.synchronize()
+    codes, start = [set(), set(), set(), set()], Barrier(4)
+
+    def work(i):
+        name, args = made[i][1]
+        fn = getattr(real, name)
+        start.wait()
+        for _ in range(5000):                            # nothing but the library's call: the threads meet inside it
+            codes[i].add(fn(*args))
+    threads = [Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{_ffi.OK}] * 4
+    assert all(torch.equal(a, res[0]) for a, (res, *_) in zip(alone, made))
