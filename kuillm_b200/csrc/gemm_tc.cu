@@ -706,10 +706,15 @@ bool encode_tmap_2byte(CUtensorMap* map, const void* base, uint32_t rank, const 
   for (uint32_t i = 0; i < rank; ++i) { gdim[i] = dims[i]; gbox[i] = box[i]; estride[i] = 1; }
   for (uint32_t i = 1; i < rank; ++i) gstride[i - 1] = strides_elems[i] * 2;
   // bf16 and f16 move identically; the type only matters for OOB fill, which is zero
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstride, gbox,
-                        estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  auto encode = [&] {
+    return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstride, gbox,
+                    estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  if (encode() == CUDA_SUCCESS) return true;
+  // a host thread that has made no call of the runtime yet has no context; setting its device gives it the device's own
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode() == CUDA_SUCCESS;
 }
 
 unsigned int* tc_error_word_device() {

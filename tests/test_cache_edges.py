@@ -55,6 +55,18 @@ def test_tree_visible_values_that_are_not_finite(cuda, n, h, hk, l, s, d, lens, 
 # ------------------------------------------------------------------------------------------------
 # host threads
 # ------------------------------------------------------------------------------------------------
+class Recorder:
+    """Makes the library's calls and keeps the arguments of the last one."""
+    def __init__(self, real):
+        self.real = real
+
+    def __getattr__(self, name):
+        def fn(*a):
+            self.last = (name, a)
+            return getattr(self.real, name)(*a)
+        return fn
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", ["tree", "mass", "sdpa"])
 def test_host_threads_with_different_head_sizes(cuda, op, monkeypatch):
@@ -74,14 +86,7 @@ def test_host_threads_with_different_head_sizes(cuda, op, monkeypatch):
         a = (r(1, 2, 16, e), r(1, 2, 32, e), r(1, 2, 32, ev))
         return lambda: _ffi.sdpa(*a)
 
-    class Recorder:
-        """Makes the library's calls and keeps the arguments of each."""
-        def __getattr__(self, name):
-            def fn(*a):
-                self.last = (name, a)
-                return getattr(real, name)(*a)
-            return fn
-    real, rec = _ffi.lib(), Recorder()
+    real, rec = _ffi.lib(), Recorder(_ffi.lib())
     monkeypatch.setattr(_ffi, "lib", lambda: rec)
     made = []                                            # per thread: result, function and arguments, and what keeps them alive
     for e in (1024, 420, 1024, 420):
@@ -111,3 +116,32 @@ def test_host_threads_with_different_head_sizes(cuda, op, monkeypatch):
     torch.cuda.synchronize()
     assert codes == [{_ffi.OK}] * 4
     assert all(torch.equal(a, res[0]) for a, (res, *_) in zip(alone, made))
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_host_thread(cuda, monkeypatch):
+    """A thread whose first use of the GPU is one of the library's calls."""
+    from threading import Thread
+    real, rec = _ffi.lib(), Recorder(_ffi.lib())
+    Q, K, V, Kd, Vd, mask = tree_inputs(1, 8, 2, 5, 300, 128, "bf16", seed=3)
+    A, B = torch.randn(64, 256, device="cuda").bfloat16(), torch.randn(128, 256, device="cuda").bfloat16()
+    lse = torch.full((1, 8, 5), 4.0, device="cuda")
+    monkeypatch.setattr(_ffi, "lib", lambda: rec)
+    made = []
+    for fn in (lambda: _ffi.gemm(A, B, trans_b=True), lambda: _ffi.sdpa(Q, K, V, is_causal=True), lambda: _ffi.sdpa(K, K, V, is_causal=True),
+               lambda: _ffi.sdpa_tree(Q, K, V, None, Kd, Vd, mask), lambda: _ffi.attn_mass(Q, K, lse)):
+        res = fn()
+        made.append((res if isinstance(res, tuple) else (res,), rec.last))
+    monkeypatch.undo()
+    torch.cuda.synchronize()
+    want = [res[0].clone() for res, _ in made]
+    for res, _ in made:
+        res[0].zero_()
+    torch.cuda.synchronize()
+    codes = []
+    for _, (name, args) in made:
+        t = Thread(target=lambda: codes.append(getattr(real, name)(*args)))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [_ffi.OK] * 5 and all(torch.equal(a, res[0]) for a, (res, _) in zip(want, made))
