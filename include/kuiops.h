@@ -391,7 +391,8 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
  * softmax weights to the element type before the product with V, as kuiops_sdpa does.
  * s may be 0 (K and V may then be NULL).  e <= 1024, ev <= 256 (KUIOPS_EUNSUPPORTED beyond),
  * l <= KUIOPS_TREE_MAX_ROWS.  workspace: kuiops_sdpa_tree_workspace_bytes(...) bytes, 16-byte aligned, no initial
- * contents required; calls that may overlap on the GPU need workspaces of their own.  out and lse overlap none of the
+ * contents required; calls that may overlap on the GPU need workspaces of their own (calls into one
+ * stream do not, whichever host threads make them).  out and lse overlap none of the
  * inputs.  No counterpart in the reference. */
 KUIOPS_API size_t kuiops_sdpa_tree_workspace_bytes(int dtype, uint32_t n, uint32_t h, uint32_t h_kv,
                                    uint32_t l, uint32_t s, uint32_t e, uint32_t ev);

@@ -6,6 +6,7 @@
 // This file holds the entry point, the SIMT kernel for every type, head dimension and stride, and the kernel that
 // joins key slices.  16-bit operands with up to 128 features per head run on the tensor cores (sdpa_tree_tc.cu).
 #include "tree.cuh"
+#include <mutex>
 
 namespace kuiops {
 
@@ -351,6 +352,11 @@ int kuiops_sdpa_tree(const kuiops_sdpa_tree_args* args, kuiops_stream_t stream) 
   const uint32_t splits = sdpa_tree_simt_splits(a);
   const size_t need = tc ? sdpa_tree_tc_workspace_bytes(a) : tree_record_bytes(a, splits);
   if (need && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace))) return KUIOPS_EWORKSPACE;
+  // A call's kernels follow each other in the stream: host threads that share a stream share its workspace, and another call's
+  // kernel between these two would overwrite the records.
+  static std::mutex launches;
+  std::unique_lock<std::mutex> lock(launches, std::defer_lock);
+  if (need) lock.lock();
   if (tc) return sdpa_tree_tc(a, st);
   float* partials = static_cast<float*>(a.workspace);
   const int run = sdpa_tree_simt(a, partials, splits, st);

@@ -145,3 +145,42 @@ def test_first_call_of_a_host_thread(cuda, monkeypatch):
         t.join()
     torch.cuda.synchronize()
     assert codes == [_ffi.OK] * 5 and all(torch.equal(a, res[0]) for a, (res, _) in zip(want, made))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,l", [("bf16", 5), ("bf16", 24), ("f32", 5)])
+def test_host_threads_on_one_stream(cuda, dtype, l, monkeypatch):
+    """Calls that leave records for a joining kernel, from several threads into one stream: they share the stream's workspace, and
+    each gets its own result."""
+    from threading import Barrier, Thread
+    real, rec = _ffi.lib(), Recorder(_ffi.lib())
+    monkeypatch.setattr(_ffi, "lib", lambda: rec)
+    made = []
+    for seed in range(3):
+        inputs = tree_inputs(1, 8, 2, l, 3000, 128, dtype, seed=seed)
+        Q, K, V, Kd, Vd, mask = inputs
+        made.append((_ffi.sdpa_tree(Q, K, V, None, Kd, Vd, mask), rec.last, inputs))
+    monkeypatch.undo()
+    torch.cuda.synchronize()
+    alone = [[t.clone() for t in res] for res, *_ in made]
+    start, wrong, codes = Barrier(3), [0, 0, 0], set()
+    for _ in range(20):
+        for res, *_ in made:
+            res[0].fill_(7.0)
+        torch.cuda.synchronize()
+
+        def work(i):
+            name, args = made[i][1]
+            fn = getattr(real, name)
+            start.wait()
+            for _ in range(100):
+                codes.add(fn(*args))
+        threads = [Thread(target=work, args=(i,)) for i in range(3)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for i, (res, *_) in enumerate(made):
+            wrong[i] += not all(torch.equal(a, b) for a, b in zip(alone[i], res))
+    assert wrong == [0, 0, 0] and codes == {_ffi.OK}
