@@ -68,7 +68,9 @@ KUIOPS_API int         kuiops_abi_version(void);
 KUIOPS_API const char* kuiops_strerror(int code);
 /* Diagnostics for the tensor-core kernels, whose pipeline waits are bounded: copies the
  * device-side error word to *host_out (0 = no wait ever ran out; otherwise the code of the
- * wait that gave up) and optionally clears it.  Synchronises the device. */
+ * wait that gave up) and optionally clears it.  Synchronises the device.  Each kernel has codes of
+ * its own: products 1 - 4, decode attention 10 - 19, prompt attention 20 - 28, the gathering norm 30,
+ * attention of drafted tokens 40 - 49, 60 and 61, attention mass 50 - 58. */
 KUIOPS_API int kuiops_debug_tc_error(unsigned int* host_out, int reset);
 /* Self-timing of the tcgen05 GEMM: while `device_buffer` (>= 32 uint64 on the current device) is set,
  * CTA 0 of every GEMM launched afterwards stores the global nanosecond timer at the stations of its

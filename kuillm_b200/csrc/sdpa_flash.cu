@@ -102,7 +102,7 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   // (two CTAs must fit one SM), so a misaligned base is reported instead of worked around.
   extern __shared__ __align__(1024) unsigned char smem[];
   if ((tc::smem_u32(smem) & 1023u) != 0) {
-    if (threadIdx.x == 0) atomicExch(p.err, 10u);
+    if (threadIdx.x == 0) atomicExch(p.err, 20u);
     return;
   }
   unsigned char* q_s = smem;
@@ -180,7 +180,7 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // Q and the first F_RING positions were requested during set-up
         for (uint32_t n = F_RING; n < 2 * n_tiles; ++n) {
           const uint32_t buf = n % F_RING, ph = (n / F_RING) & 1;
-          if (!flash_wait(&t_empty[buf], ph ^ 1)) { atomicExch(p.err, 11u); break; }
+          if (!flash_wait(&t_empty[buf], ph ^ 1)) { atomicExch(p.err, 21u); break; }
           unsigned char* dst = ring + buf * F_T_BYTES;
           const CUtensorMap* tm = (n & 1) ? &tmV : &tmK;
           const int key0 = int((n >> 1) * FBN);
@@ -196,13 +196,13 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         constexpr uint32_t idesc_qk = tc::make_idesc(is_bf16, 0, 0, FBM, FBN);
         constexpr uint32_t idesc_pv = tc::make_idesc(is_bf16, 0, 1, FBM, FD);
         bool ok = flash_wait(q_full, 0);
-        if (!ok) atomicExch(p.err, 12u);
+        if (!ok) atomicExch(p.err, 22u);
         const uint32_t qa = tc::smem_u32(q_s);
         // S = Q K^T of tile j into S buffer j & 1: two 64-wide halves of the head dim x four 16-wide steps
         auto issue_qk = [&](uint32_t j) -> bool {
           const uint32_t n = 2 * j, buf = n % F_RING, ph = (n / F_RING) & 1;
           const uint32_t ka = tc::smem_u32(ring + buf * F_T_BYTES);
-          if (!flash_wait(&t_full[buf], ph)) { atomicExch(p.err, 13u); return false; }
+          if (!flash_wait(&t_full[buf], ph)) { atomicExch(p.err, 23u); return false; }
           tc::tc_fence_after();
   #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
@@ -224,8 +224,8 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           // buffer holds P of tile j - 1; the UMMA that reads it was issued before this one and the
           // pipe runs in order, and the softmax warps left it when p_ready of tile j - 1 arrived.
           if (j + 1 < n_tiles && !issue_qk(j + 1)) { ok = false; break; }
-          if (!flash_wait(p_ready, j & 1)) { atomicExch(p.err, 14u); ok = false; break; }
-          if (!flash_wait(&t_full[buf], ph)) { atomicExch(p.err, 15u); ok = false; break; }
+          if (!flash_wait(p_ready, j & 1)) { atomicExch(p.err, 24u); ok = false; break; }
+          if (!flash_wait(&t_full[buf], ph)) { atomicExch(p.err, 25u); ok = false; break; }
           tc::tc_fence_after();
           // O += P V over the 64 keys of the tile: four 16-key steps; P (16 keys = 8 TMEM columns of
           // the S buffer the softmax overwrote) from TMEM, V MN-major (head dim contiguous)
@@ -251,7 +251,7 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     float m_used = -INFINITY, l_run = 0.f;
     bool ok = true;
     for (uint32_t j = 0; j < n_tiles && ok; ++j) {
-      if (!flash_wait(&s_full[j & 1], (j >> 1) & 1)) { atomicExch(p.err, 16u); ok = false; break; }
+      if (!flash_wait(&s_full[j & 1], (j >> 1) & 1)) { atomicExch(p.err, 26u); ok = false; break; }
       tc::tc_fence_after();
       float sv[FBN];
       tc::tmem_ld32(tmem_S + (j & 1) * FBN + lane_addr, sv);
@@ -303,7 +303,7 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // when nothing depends on it: a parity wait only tells the current phase of the barrier from the one before, so
         // every phase has to be observed in turn.  The wait sits after this tile's exponentials,
         // by which time that UMMA has normally completed.
-        if (!flash_wait(o_done, (j - 1) & 1)) { atomicExch(p.err, 17u); ok = false; break; }
+        if (!flash_wait(o_done, (j - 1) & 1)) { atomicExch(p.err, 27u); ok = false; break; }
         tc::tc_fence_after();
       }
       if (rescale) {
@@ -327,7 +327,7 @@ sdpa_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (lane == 0) tc::mbar_arrive(p_ready);
     }
     if (ok && n_tiles > 0) {
-      if (!flash_wait(o_done, (n_tiles - 1) & 1)) { atomicExch(p.err, 18u); ok = false; }
+      if (!flash_wait(o_done, (n_tiles - 1) & 1)) { atomicExch(p.err, 28u); ok = false; }
     }
     if (ok) {
       tc::tc_fence_after();

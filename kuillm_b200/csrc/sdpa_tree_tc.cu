@@ -340,7 +340,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           for (uint32_t half = 0; half < TT::kHalves; ++half)
             tc::tma_load_4d(dst + half * (RTN * 128), tm, &t_full[buf], int(half * 64), key0, int(seg.skvh), int(seg.sb));
           if (i + 1 == early) {
-            if (n_seg > 0 && !tree_wait(q_empty, (n_seg - 1) & 1)) { atomicCAS(p.err, 0u, 50u); ok = false; ++n; break; }
+            if (n_seg > 0 && !tree_wait(q_empty, (n_seg - 1) & 1)) { atomicCAS(p.err, 0u, 60u); ok = false; ++n; break; }
             tc::mbar_expect_tx(q_full, REP * TT::kHalves * p.rows * 128u);
 #pragma unroll
             for (uint32_t half = 0; half < TT::kHalves; ++half)
@@ -397,7 +397,7 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (!tree_wait(p_ready, g & 1)) { atomicCAS(p.err, 0u, 44u); ok = false; break; }
           if (!tree_wait(&t_full[buf], (n / R) & 1)) { atomicCAS(p.err, 0u, 45u); ok = false; break; }
           // a new segment's O overwrites the one before, which has to have been read
-          if (j == 0 && n_seg > 0 && !tree_wait(o_free, (n_seg - 1) & 1)) { atomicCAS(p.err, 0u, 51u); ok = false; break; }
+          if (j == 0 && n_seg > 0 && !tree_wait(o_free, (n_seg - 1) & 1)) { atomicCAS(p.err, 0u, 61u); ok = false; break; }
           tc::tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)

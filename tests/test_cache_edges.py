@@ -1,5 +1,8 @@
 """Values, layouts, sizes and threads at which the operators on a KV cache can go wrong and that the tests of their ordinary
 range do not reach.  Error bounds as in test_cache_ops.py."""
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -7,6 +10,15 @@ import torch
 from kuipy import _ffi
 from oracle import kuiops_oracle as O
 from test_cache_ops import check_tree, f64, lens_t, tree_inputs
+
+
+def test_error_codes_name_one_kernel():
+    """The error word says which wait gave up: no two kernels share a code."""
+    owner = {}
+    for src in sorted((Path(_ffi.__file__).resolve().parents[1] / "csrc").glob("*.cu*")):
+        for code in re.findall(r"atomic(?:CAS\(\s*(?:p\.)?err, 0u|Exch\((?:p\.)?err), (\d+)u", src.read_text()):
+            assert owner.setdefault(int(code), src.name) == src.name, (code, owner[int(code)], src.name)
+    assert len(set(owner.values())) >= 6
 
 
 # ------------------------------------------------------------------------------------------------
