@@ -414,6 +414,8 @@ class Decoder:
     def prefill(self, ids, local_logits=False):
         B, S = ids.shape
         assert self.k_cache is not None and S <= self.cap and self.length == 0 and self.kv_lens is None
+        if self.mass is not None:
+            self.mass.zero_()                   # what an earlier prompt in this cache gathered
         positions = torch.arange(S, device=self.device).repeat(B)
         if self.tp_size > 1 and B % 2 == 0 and B * S >= self.overlap_min_rows and B * S > self.exchange_rows and self.mass is None:
             out = self._forward_tp_overlap(ids, positions, S)
