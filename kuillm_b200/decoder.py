@@ -149,7 +149,7 @@ class Decoder:
         if tp_size > 1:
             self.lm_head = shard_out_features(self.lm_head, cfg.vocab, 1, tp_rank, tp_size).clone()   # a copy: the slice would keep all rows alive
         self.vocab_lo = tp_rank * (cfg.vocab // tp_size)
-        self.k_cache = self.v_cache = None
+        self.k_cache = self.v_cache = self._graph = None
         self.mass = self.kv_lens = None
         self.cap = 0
         self.length = 0
@@ -189,6 +189,7 @@ class Decoder:
         self.v_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
         self.cap, self.length, self.batch = capacity, 0, batch
         self.kv_lens = self.next_pos = self.slot_pos = None
+        self._graph = None                      # a captured step works on the cache it was captured with
         self.mass_window = int(window)
         rows = (self.cfg.n_layers * batch, self.hk, capacity)
         self.mass = torch.zeros(rows, device=self.device, dtype=torch.float32) if track_mass else None
@@ -577,6 +578,8 @@ class Decoder:
         """Run `steps` captured decode steps starting from token `first_tok` at the current length."""
         assert self.kv_lens is None, "the cache is no longer position by slot: go on with verify (a tree of one node)"
         B = first_tok.shape[0]
+        if self._graph is None or B != self._tok.shape[0]:
+            raise ValueError("decode_graph: capture_decode this batch on the present cache first")
         if out is None:
             out = torch.empty((B, steps), dtype=torch.int64, device=self.device)
         self._tok.copy_(first_tok)
@@ -600,7 +603,7 @@ class Decoder:
             return torch.stack(out, 1)
         tok = self.next_token(self.prefill(ids, local_logits=True))
         if use_graph and new_tokens > 1:
-            if getattr(self, "_graph", None) is None or self._tok.shape[0] != ids.shape[0]:
+            if self._graph is None or self._tok.shape[0] != ids.shape[0]:
                 self.capture_decode(ids.shape[0])
             rest = self.decode_graph(tok, new_tokens - 1)
             return torch.cat([tok[:, None], rest], 1)
