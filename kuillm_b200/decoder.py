@@ -183,7 +183,7 @@ class Decoder:
     # ---- state ---------------------------------------------------------------------------
     def alloc_cache(self, batch, capacity, track_mass=False, window=64):
         """track_mass: accumulate the attention weight every cache slot receives, from the last `window` rows of the prompt
-        and from every verified step on (what ``evict`` goes by)."""
+        and from every token decoded or verified after it (what ``evict`` goes by)."""
         shape = (self.cfg.n_layers, batch, self.hk, capacity, self.cfg.head_dim)
         self.k_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
         self.v_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
@@ -233,6 +233,11 @@ class Decoder:
             tiles = _ffi.ssq_tiles(cfg.d_model)
             ssq_a = torch.empty((tiles, rows), dtype=torch.float32, device=self.device)
             ssq_b = torch.empty((tiles, rows), dtype=torch.float32, device=self.device)
+        observe = self.mass is not None
+        if observe:
+            # a prompt's last rows vote for its slots, as a window of observation; a decoded token for all it sees
+            voters = min(seq, self.mass_window) if start == 0 else seq
+            voter_lens = torch.full((B,), end, dtype=torch.int64, device=self.device) if kv_lens is None else kv_lens
         folded_resid = False                    # True once resid holds the running sum and ssq_a its squares
         for li, L in enumerate(self.layers):
             qkv = None
@@ -268,14 +273,10 @@ class Decoder:
             else:
                 k4 = self.k_cache[li][:, :, :end]
                 v4 = self.v_cache[li][:, :, :end]
-            observe = self.mass is not None and start == 0
             lse = _ffi.sdpa(q4, k4, v4, is_causal=True, need_lse=observe, out=o4, kv_lens=kv_lens)[1]
             if observe:
-                # the prompt's last rows vote for its slots, as a window of observation
-                w = min(seq, self.mass_window)
                 mass = self.mass[li * B:(li + 1) * B]
-                _ffi.attn_mass(q4[:, :, seq - w:], self.k_cache[li], lse[:, :, seq - w:], kv_lens=torch.full((B,), seq, dtype=torch.int64, device=self.device),
-                               is_causal=True, mass=mass, out=mass)
+                _ffi.attn_mass(q4[:, :, seq - voters:], self.k_cache[li], lse[:, :, seq - voters:], kv_lens=voter_lens, is_causal=True, mass=mass, out=mass)
             if fold and (folded_resid or _ffi.gemm_residual_ssq(attn, L["wo"], resid, ssq_b)):
                 if folded_resid:
                     _ffi.gemm_residual_ssq(attn, L["wo"], resid, ssq_b)          # resid += attn Wo^T, squares -> ssq_b
@@ -553,6 +554,7 @@ class Decoder:
         self._pos = torch.zeros(batch, dtype=torch.int64, device=dev)
         self._kvlen = torch.ones(batch, dtype=torch.int64, device=dev)
         saved = self.length
+        votes = None if self.mass is None else self.mass.clone()
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
@@ -564,6 +566,8 @@ class Decoder:
                 self._kvlen.fill_(self.cap)
                 self._graph_step()
         torch.cuda.current_stream(dev).wait_stream(side)
+        if votes is not None:
+            self.mass.copy_(votes)              # the warm-up's tokens are none of the sequences'
         torch.cuda.synchronize(dev)
         self._graph = torch.cuda.CUDAGraph()
         self.length = 1

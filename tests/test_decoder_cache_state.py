@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from kuillm_b200.decoder import Decoder, DecoderConfig
+from kuillm_b200.decoder import Decoder, DecoderConfig, TreePlan
 from test_decoder_tree import _decoder
 
 
@@ -45,3 +45,36 @@ def test_captured_generation_in_a_new_cache(cuda):
         assert torch.equal(dec.generate(ids, 6, use_graph=True), want)
         dec.length = 0
         assert torch.equal(dec.generate(ids, 6, use_graph=True), want)           # the same capture again
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decoded_tokens_give_attention_weight_like_verified_ones(cuda, hd):
+    """A token decoded step by step, eagerly or from the captured step, adds what a verified tree of one node adds."""
+    g = torch.Generator().manual_seed(5)
+    ids, toks = torch.randint(0, 1000, (2, 12), generator=g).cuda(), torch.randint(0, 1000, (2, 4), generator=g).cuda()
+    tree, step = _decoder(hd, seed=6), _decoder(hd, seed=6)
+    rows = 2 * tree.hq * tree.cfg.n_layers                             # each spreads a weight of one over what it sees
+    for d in (tree, step):
+        d.alloc_cache(2, 32, track_mass=True, window=4)
+        d.prefill(ids)
+    assert torch.equal(tree.mass, step.mass)
+    for t in range(4):
+        before = float(step.mass.sum())
+        tree.verify(toks[:, t:t + 1], TreePlan.chain(1))
+        step.decode_step(toks[:, t])
+        assert abs(float(step.mass.sum()) - before - rows) < 2e-2 * rows
+    # both attend in 16 bits: a score is off by about one step of its 16-bit operands (2^-8 of a few units), and so is a weight
+    assert (tree.mass - step.mass).abs().max() <= 2.0 ** -4 * float(tree.mass.max())
+    assert float(step.mass[:, :, 16:].abs().max()) == 0.0
+    # the captured step: its warm-up leaves the weight alone, and every replay adds its tokens'
+    before = step.mass.clone()
+    step.capture_decode(2)
+    assert torch.equal(step.mass, before)
+    step.decode_graph(toks[:, 0], 3)
+    assert abs(float(step.mass.sum() - before.sum()) - 3 * rows) < 2e-2 * 3 * rows
+    assert float(step.mass[:, :, 15 + 4:].abs().max()) == 0.0 and float((step.mass - before).min()) >= 0.0
+    step.evict(10, sinks=2, recent=3)
+    assert step.kv_lens.tolist() == [10, 10] and step.next_pos.tolist() == [19, 19]
+    kept = step.slot_pos[:, :, :10]
+    assert bool(((kept >= 3) & (kept < 16)).any())
