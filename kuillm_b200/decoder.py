@@ -439,18 +439,25 @@ class Decoder:
         B = self.batch
         self.kv_lens = torch.full((B,), self.length, dtype=torch.int64, device=self.device)
         self.next_pos = self.kv_lens.clone()
+        self._used = self.length                # at least as many slots as any sequence has in use
         self.slot_pos = torch.arange(self.cap, dtype=torch.int32, device=self.device).expand(self.cfg.n_layers * B, self.hk, self.cap).contiguous()
 
     def verify(self, tokens, plan, return_logits=False):
         """One step over a tree: tokens [B, plan.size], node 0 the token that is certain (the last one accepted), the others drafted
         below it.  One pass scores every node, the greedy path through the tree is accepted and its keys and values go to the
         cache.  Returns (path [B, size] of accepted nodes, then -1; counts [B]; next token [B]), and the logits [B, size,
-        vocab / tp] if asked.  The caller keeps room: counts are at most plan.max_depth, kv_lens + max_depth at most the capacity."""
+        vocab / tp] if asked.  A sequence may grow by plan.max_depth slots: without room for them in each (kv_lens + max_depth
+        beyond the capacity) the step is refused before it starts."""
         cfg, B, l = self.cfg, tokens.shape[0], plan.size
         if self.k_cache is None or B != self.batch or tokens.shape[1] != l:
             raise ValueError("verify: tokens [batch, plan.size] on an allocated cache")
         if self.kv_lens is None:
             self._start_ragged()
+        if self._used + plan.max_depth > self.cap:
+            self._used = int(self.kv_lens.max())            # the host counts every step's whole depth: look at what was accepted
+            if self._used + plan.max_depth > self.cap:
+                raise ValueError(f"verify: {self._used} of {self.cap} slots are in use, a step may take {plan.max_depth}: evict first")
+        self._used += plan.max_depth
         hd, hq, hk, rows = cfg.head_dim, self.hq, self.hk, B * l
         W = (hq + 2 * hk) * hd
         positions = (self.next_pos[:, None] + plan.depth).reshape(-1)
@@ -506,6 +513,7 @@ class Decoder:
         K, V = (c.reshape(n, self.hk, self.cap, self.cfg.head_dim) for c in (self.k_cache, self.v_cache))
         self.kv_lens, self.mass, self.slot_pos, src = _ffi.kv_evict(K, V, self.mass, self.kv_lens, budget, pos=self.slot_pos, next_pos=self.next_pos,
                                                                     sinks=sinks, recent=recent)
+        self._used = min(self._used, budget)
         return src
 
     def generate_tree(self, ids, new_tokens, plan, propose, budget=None, sinks=4, recent=64):

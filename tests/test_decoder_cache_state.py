@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from kuipy import _ffi
 from kuillm_b200.decoder import Decoder, DecoderConfig, TreePlan
 from test_decoder_tree import _decoder
 
@@ -78,3 +79,30 @@ def test_decoded_tokens_give_attention_weight_like_verified_ones(cuda, hd):
     assert step.kv_lens.tolist() == [10, 10] and step.next_pos.tolist() == [19, 19]
     kept = step.slot_pos[:, :, :10]
     assert bool(((kept >= 3) & (kept < 16)).any())
+
+
+@pytest.mark.gpu
+def test_a_step_that_may_not_fit_is_refused(cuda):
+    """The cache may be filled to its last slot; a step that could pass it changes nothing, and an eviction makes room again."""
+    dec = _decoder(64, seed=7)
+    ids = torch.randint(0, 1000, (2, 9), generator=torch.Generator().manual_seed(8)).cuda()
+    tree = TreePlan([-1, 0, 0, 1])                                      # up to three slots
+    dec.alloc_cache(2, 16, track_mass=True, window=4)
+    last = dec.next_token(dec.prefill(ids))
+    wrong = torch.full((2, 3), 1000 - 1, dtype=torch.int64, device="cuda")
+    steps = 0
+    while int(dec.kv_lens.max()) + 3 <= 16 if dec.kv_lens is not None else True:      # rejected drafts take one slot a step
+        _, counts, last = dec.verify(torch.cat([last[:, None], wrong], 1), tree)
+        steps += 1
+    assert steps >= 2
+    state = [t.clone() for t in (dec.kv_lens, dec.next_pos, dec.mass, dec.slot_pos, dec.k_cache)]
+    with pytest.raises(ValueError):
+        dec.verify(torch.cat([last[:, None], wrong], 1), tree)
+    assert all(torch.equal(a, b) for a, b in zip(state, (dec.kv_lens, dec.next_pos, dec.mass, dec.slot_pos, dec.k_cache)))
+    while int(dec.kv_lens.max()) < 16:                                  # single nodes go on to the last slot
+        _, _, last = dec.verify(last[:, None], TreePlan.chain(1))
+    with pytest.raises(ValueError):
+        dec.verify(last[:, None], TreePlan.chain(1))
+    dec.evict(10, sinks=2, recent=3)
+    _, counts, _ = dec.verify(torch.cat([last[:, None], wrong], 1), tree)
+    assert dec.kv_lens.tolist() == (10 + counts).tolist() and _ffi.check_status(torch.device("cuda", 0)) == 0
