@@ -415,7 +415,8 @@ class Decoder:
 
     def prefill(self, ids, local_logits=False):
         B, S = ids.shape
-        assert self.k_cache is not None and S <= self.cap and self.length == 0 and self.kv_lens is None
+        self._slots_are_positions("prefill")
+        assert self.k_cache is not None and S <= self.cap and self.length == 0
         if self.mass is not None:
             self.mass.zero_()                   # what an earlier prompt in this cache gathered
         positions = torch.arange(S, device=self.device).repeat(B)
@@ -427,12 +428,18 @@ class Decoder:
 
     def decode_step(self, ids, local_logits=False):
         B = ids.shape[0]
-        assert self.kv_lens is None, "the cache is no longer position by slot: go on with verify (a tree of one node)"
+        self._slots_are_positions("decode_step")
         positions = torch.full((B,), self.length, device=self.device, dtype=torch.int64)
         out = self._forward(ids.reshape(B, 1), positions, 1)
         return out if local_logits else self._full_logits(out)
 
     # ---- trees of drafted tokens, bounded cache --------------------------------------------------
+    def _slots_are_positions(self, what):
+        """Guards the paths that take a slot of the cache for its token's position (an exception, not an assert statement: it stays
+        when Python runs optimised)."""
+        if self.kv_lens is not None:
+            raise AssertionError(f"{what}: after verify or evict the cache is no longer position by slot; go on with verify (a tree of one node)")
+
     def _start_ragged(self):
         """The cache as `prefill` and `decode_step` left it, seen per sequence: slots in use, the next token's position, and each
         slot's position."""
@@ -555,7 +562,7 @@ class Decoder:
 
     def capture_decode(self, batch):
         """Capture the decode step in a CUDA graph (launch-bound otherwise: ~290 kernels per token)."""
-        assert self.kv_lens is None, "the capture's warm-up writes the last slot, which may be in use after verify or evict"
+        self._slots_are_positions("capture_decode")
         dev = self.device
         self._tok = torch.zeros(batch, dtype=torch.int64, device=dev)
         self._tok_out = torch.zeros(batch, dtype=torch.int64, device=dev)
@@ -588,7 +595,7 @@ class Decoder:
 
     def decode_graph(self, first_tok, steps, out=None):
         """Run `steps` captured decode steps starting from token `first_tok` at the current length."""
-        assert self.kv_lens is None, "the cache is no longer position by slot: go on with verify (a tree of one node)"
+        self._slots_are_positions("decode_graph")
         B = first_tok.shape[0]
         if self._graph is None or B != self._tok.shape[0]:
             raise ValueError("decode_graph: capture_decode this batch on the present cache first")

@@ -1,8 +1,13 @@
 """What the decoder keeps beside its cache - attention weight, slots in use, the captured step - through every order of calls."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
-from kuipy import _ffi
+from kuillm_b200.kuipy import _ffi
 from kuillm_b200.decoder import Decoder, DecoderConfig, TreePlan
 from test_decoder_tree import _decoder
 
@@ -106,3 +111,23 @@ def test_a_step_that_may_not_fit_is_refused(cuda):
     dec.evict(10, sinks=2, recent=3)
     _, counts, _ = dec.verify(torch.cat([last[:, None], wrong], 1), tree)
     assert dec.kv_lens.tolist() == (10 + counts).tolist() and _ffi.check_status(torch.device("cuda", 0)) == 0
+
+
+def test_guards_hold_when_python_runs_optimised():
+    code = """
+import torch
+from test_decoder_cache_state import _cpu_decoder
+dec = _cpu_decoder()
+dec.alloc_cache(1, 8)
+dec.kv_lens = torch.zeros(1, dtype=torch.int64)
+ids = torch.zeros(1, 1, dtype=torch.int64)
+for call in (lambda: dec.prefill(ids), lambda: dec.decode_step(ids[0]), lambda: dec.capture_decode(1), lambda: dec.decode_graph(ids[0], 1)):
+    try:
+        call()
+    except AssertionError as e:
+        print("refused:", e)
+"""
+    tests = Path(__file__).resolve().parent
+    env = {**os.environ, "PYTHONPATH": os.pathsep.join(str(p) for p in (tests, tests.parent, tests.parent / "kuillm_b200"))}
+    r = subprocess.run([sys.executable, "-O", "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.stdout.count("refused:") == 4, r.stdout + r.stderr
