@@ -184,6 +184,8 @@ class Decoder:
     def alloc_cache(self, batch, capacity, track_mass=False, window=64):
         """track_mass: accumulate the attention weight every cache slot receives, from the last `window` rows of the prompt
         and from every token decoded or verified after it (what ``evict`` goes by)."""
+        if window < 0:
+            raise ValueError("alloc_cache: a window of prompt rows, or none")
         shape = (self.cfg.n_layers, batch, self.hk, capacity, self.cfg.head_dim)
         self.k_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
         self.v_cache = torch.zeros(shape, device=self.device, dtype=self.cfg.dtype)
@@ -237,6 +239,7 @@ class Decoder:
         if observe:
             # a prompt's last rows vote for its slots, as a window of observation; a decoded token for all it sees
             voters = min(seq, self.mass_window) if start == 0 else seq
+            observe = voters > 0                # a window of none: only what is decoded votes
             voter_lens = torch.full((B,), end, dtype=torch.int64, device=self.device) if kv_lens is None else kv_lens
         folded_resid = False                    # True once resid holds the running sum and ssq_a its squares
         for li, L in enumerate(self.layers):

@@ -131,3 +131,18 @@ for call in (lambda: dec.prefill(ids), lambda: dec.decode_step(ids[0]), lambda: 
     env = {**os.environ, "PYTHONPATH": os.pathsep.join(str(p) for p in (tests, tests.parent, tests.parent / "kuillm_b200"))}
     r = subprocess.run([sys.executable, "-O", "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert r.stdout.count("refused:") == 4, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+def test_a_window_of_no_prompt_rows(cuda):
+    """Without a window the prompt gives no weight, the tokens after it do."""
+    dec = _decoder(64, seed=9)
+    ids = torch.randint(0, 1000, (2, 9), generator=torch.Generator().manual_seed(8)).cuda()
+    dec.alloc_cache(2, 16, track_mass=True, window=0)
+    last = dec.next_token(dec.prefill(ids))
+    assert float(dec.mass.abs().max()) == 0.0
+    dec.decode_step(last)
+    rows = 2 * dec.hq * dec.cfg.n_layers
+    assert abs(float(dec.mass.sum()) - rows) < 2e-2 * rows
+    with pytest.raises(ValueError):
+        dec.alloc_cache(2, 16, track_mass=True, window=-1)
