@@ -608,7 +608,18 @@ def _own_rows(t):
     """A 4-D tensor that rows can be written to one by one: contiguous innermost, no two rows the same memory."""
     n, hkv, rows, e = t.shape
     a, b, c, d = t.stride()
-    return (e == 1 or d == 1) and (rows == 1 or c >= e) and (hkv == 1 or b >= e) and (n == 1 or a >= e)
+    if e > 1 and d != 1:
+        return False
+    if c >= e and b >= c * rows and a >= b * hkv:          # the common order of dimensions
+        return True
+    # from the closest dimension outwards each has to step over all that lies within
+    reach = e
+    for step, size in sorted(((c, rows), (b, hkv), (a, n))):
+        if size > 1:
+            if step < reach:
+                return False
+            reach += step * (size - 1)
+    return True
 
 
 def _dense(t, dtype, what):

@@ -196,3 +196,24 @@ def test_host_threads_on_one_stream(cuda, dtype, l, monkeypatch):
         for i, (res, *_) in enumerate(made):
             wrong[i] += not all(torch.equal(a, b) for a, b in zip(alone[i], res))
     assert wrong == [0, 0, 0] and codes == {_ffi.OK}
+
+
+# ------------------------------------------------------------------------------------------------
+# layouts that are written to
+# ------------------------------------------------------------------------------------------------
+def test_rows_that_share_memory_are_not_written():
+    """A cache or output whose (entry, head, row) steps coincide has rows on top of each other; dense ones in any order of dimensions,
+    slices and gaps do not."""
+    flat = torch.zeros(4096)
+    view = lambda shape, stride: flat.as_strided(shape, stride)                                  # noqa: E731
+    for shape, stride in (((2, 3, 5, 8), (120, 40, 8, 1)), ((2, 3, 5, 8), (120, 8, 24, 1)), ((2, 3, 5, 8), (8, 80, 16, 1)), ((2, 3, 5, 8), (400, 50, 9, 1)),
+                          ((1, 3, 5, 8), (0, 40, 8, 1)), ((2, 1, 5, 8), (40, 0, 8, 1)), ((2, 3, 1, 8), (24, 8, 0, 1)), ((2, 3, 5, 1), (15, 5, 1, 7)),
+                          ((1, 1, 1, 8), (0, 0, 0, 1))):
+        assert _ffi._own_rows(view(shape, stride)), stride
+    for shape, stride in (((2, 3, 5, 8), (8, 8, 8, 1)), ((2, 3, 5, 8), (120, 8, 8, 1)), ((2, 3, 5, 8), (40, 40, 8, 1)), ((2, 3, 5, 8), (120, 39, 8, 1)),
+                          ((2, 3, 5, 8), (119, 40, 8, 1)), ((2, 3, 5, 8), (0, 40, 8, 1)), ((2, 3, 5, 8), (120, 40, 8, 2)), ((2, 3, 5, 8), (120, 40, 7, 1))):
+        t = view(shape, stride)
+        assert not _ffi._own_rows(t), stride
+        with pytest.raises(_ffi.KuiopsError) as err:
+            _ffi.kv_append(t, t, torch.zeros(2, dtype=torch.int64), t, t)
+        assert "rows of their own" in str(err.value)
