@@ -9,7 +9,7 @@ import torch
 
 from kuipy import _ffi
 from oracle import kuiops_oracle as O
-from test_cache_ops import check_tree, f64, lens_t, tree_inputs
+from test_cache_ops import DT, check_evict, check_mass, check_tree, f64, lens_t, tree_inputs
 
 
 def test_error_codes_name_one_kernel():
@@ -217,3 +217,91 @@ def test_rows_that_share_memory_are_not_written():
         with pytest.raises(_ffi.KuiopsError) as err:
             _ffi.kv_append(t, t, torch.zeros(2, dtype=torch.int64), t, t)
         assert "rows of their own" in str(err.value)
+
+
+# ------------------------------------------------------------------------------------------------
+# eviction whose moves take a launch of their own (more than 16 MiB could move)
+# ------------------------------------------------------------------------------------------------
+def evict_inputs(n, hk, cap, d, dv, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if dtype == "u8":
+        r = lambda *s: torch.randint(0, 256, s, generator=g, device="cuda", dtype=torch.uint8)  # noqa: E731
+    else:
+        r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(DT[dtype])                 # noqa: E731
+    return r, torch.exp(2 * torch.randn(n, hk, cap, generator=g, device="cuda"))
+
+
+def spreads(n, hk, cap, budget, d, dv, size):
+    return n * hk * min(budget, cap - budget) * (d + dv) * size > 16 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,hk,cap,budget,d,dv,dtype,lens,sinks,recent", [
+    (6, 8, 2500, 1001, 128, 128, "bf16", [2500, 900, 0], 4, 64),           # a budget of no whole chunks, several layers, rows within it
+    (4, 8, 2200, 1056, 128, 128, "f16", [2200, 1056, 1057, 1 << 40], 0, 0),
+    (2, 4, 9000, 4097, 128, 128, "bf16", [9000, 4098], 1, 4096),
+    (16, 8, 700, 257, 128, 64, "f32", [700, 258, 600, 257], 0, 257),
+    (4, 4, 30000, 14001, 33, 7, "bf16", [29999, 14002], 2, 100),           # 2-byte units
+    (4, 2, 17000, 8191, 37, 35, "f32", [17000], 0, 8191),                  # 4-byte units
+    (4, 2, 24000, 11003, 100, 101, "u8", [23000, 24000], 4, 10),           # single bytes
+])
+def test_evict_moves_in_a_launch_of_their_own(cuda, n, hk, cap, budget, d, dv, dtype, lens, sinks, recent):
+    r, mass = evict_inputs(n, hk, cap, d, dv, dtype, budget)
+    K, V = r(n, hk, cap, d), r(n, hk, cap, dv)
+    assert spreads(n, hk, cap, budget, d, dv, K.element_size())
+    check_evict(K, V, mass, lens, budget, sinks=sinks, recent=recent)
+
+
+@pytest.mark.gpu
+def test_evict_moves_in_a_launch_of_their_own_strides_and_positions(cuda):
+    """Rows off the 16-byte grid, slices, (entry, slot, head) order, and positions out of order as earlier evictions leave them."""
+    n, hk, cap, budget, d = 4, 4, 5000, 2177, 128
+    r, mass = evict_inputs(n, hk, cap, d, d, "bf16", 1)
+    assert spreads(n, hk, cap, budget, d, d, 2)
+    pos = torch.stack([torch.randperm(9000, generator=torch.Generator().manual_seed(i))[:cap] for i in range(n * hk)]).view(n, hk, cap).int().cuda()
+    V = r(n, cap, hk, d).transpose(1, 2)
+    for K in (r(n, hk, cap + 9, d)[:, :, 9:], r(n * hk * cap * d + 1)[1:].view(n, hk, cap, d), r(n, hk, cap, d + 1)[..., 1:]):
+        check_evict(K, V.clone(), mass, [5000, 3001], budget, pos=pos, next_pos=[9000, 9000], sinks=30, recent=500)
+
+
+@pytest.mark.gpu
+def test_evict_moves_in_a_launch_of_their_own_captured(cuda):
+    n, hk, cap, budget, d = 5, 8, 2500, 1001, 128
+    r, mass = evict_inputs(n, hk, cap, d, d, "bf16", 2)
+    K0, V0 = r(n, hk, cap, d), r(n, hk, cap, d)
+    assert spreads(n, hk, cap, budget, d, d, 2)
+    K, V, lens = K0.clone(), V0.clone(), lens_t([2500])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = _ffi.kv_evict(K, V, mass, lens, budget, sinks=4, recent=64)
+    for k, change in enumerate(([2500], [1001], [2111])):
+        K.copy_(K0)
+        V.copy_(V0)
+        lens.copy_(lens_t(change))
+        mass.copy_(mass.roll(k + 1, 2))
+        graph.replay()
+        torch.cuda.synchronize()
+        K1, V1 = K0.clone(), V0.clone()
+        want = _ffi.kv_evict(K1, V1, mass, lens, budget, sinks=4, recent=64)
+        assert all(torch.equal(a, b) for a, b in zip(got + (K, V), want + (K1, V1)))
+    del graph
+
+
+@pytest.mark.gpu
+def test_evict_offsets_beyond_32_bits(cuda):
+    """The last entry's rows lie 2^31 elements behind the first one's."""
+    n, hk, cap, budget, d, used = 3, 8, 1 << 20, 2003, 128, 2600
+    K, V = (torch.empty(n, hk, cap, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    mass = torch.zeros(n, hk, cap, device="cuda")
+    r, m = evict_inputs(1, hk, used, d, d, "bf16", 3)
+    k, v = r(1, hk, used, d), r(1, hk, used, d)
+    K[2:, :, :used], V[2:, :, :used], mass[2:, :, :used] = k, v, m
+    assert spreads(n, hk, cap, budget, d, d, 2)
+    lens, mass_out, pos, src = _ffi.kv_evict(K, V, mass, lens_t([0, 0, used]), budget, sinks=4, recent=100)
+    want = _ffi.kv_evict(k, v, m, lens_t([used]), budget, sinks=4, recent=100)
+    assert lens.tolist() == [0, 0, budget] and torch.equal(src[2:], want[3]) and bool((src[:2] == -1).all())
+    assert torch.equal(K[2:, :, :used], k) and torch.equal(V[2:, :, :used], v)
+    assert torch.equal(mass_out[2:, :, :used], want[1]) and torch.equal(pos[2:, :, :used], want[2])
+    assert float(mass_out[:, :, used:].abs().max()) == 0.0 and bool((pos[:, :, used:] == -1).all())
