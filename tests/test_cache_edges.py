@@ -305,3 +305,48 @@ def test_evict_offsets_beyond_32_bits(cuda):
     assert torch.equal(K[2:, :, :used], k) and torch.equal(V[2:, :, :used], v)
     assert torch.equal(mass_out[2:, :, :used], want[1]) and torch.equal(pos[2:, :, :used], want[2])
     assert float(mass_out[:, :, used:].abs().max()) == 0.0 and bool((pos[:, :, used:] == -1).all())
+
+
+# ------------------------------------------------------------------------------------------------
+# attention mass with a limit per row, as a verified step asks for it
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("layers,g,h,hk,l,s,d,dtype", [
+    (3, 2, 8, 2, 17, 300, 128, "bf16"),               # 68 rows a KV head: one tile of rows that streams
+    (2, 3, 32, 8, 27, 700, 128, "f16"),               # 108
+    (4, 1, 8, 2, 32, 129, 64, "bf16"),                # 128
+    (2, 2, 8, 2, 33, 260, 128, "bf16"),               # two tiles
+    (2, 3, 6, 2, 200, 150, 64, "f16"),                # five tiles, fewer keys than rows
+    (1, 2, 7, 1, 64, 1000, 80, "bf16"),               # 448 rows under seven heads
+    (32, 1, 32, 8, 27, 130, 128, "bf16"),             # every layer of a deep model
+    (2, 2, 8, 2, 20, 200, 64, "f32"),
+])
+def test_attn_mass_row_limits_with_many_rows(cuda, layers, g, h, hk, l, s, d, dtype):
+    """Most rows count for nothing (nodes that were not accepted), some for a few keys, some for more than there are; one sequence
+    counts for none at all; entry b of the layers uses limits b % g."""
+    n = layers * g
+    gen = torch.Generator().manual_seed(l + s)
+    qkv = torch.randn(n * l, (h + 2 * hk) * d, generator=gen).to(DT[dtype]).cuda()
+    Q = qkv.as_strided((n, h, l, d), (l * qkv.shape[1], d, qkv.shape[1], 1))
+    K = torch.randn(n, hk, s, d, generator=gen).to(DT[dtype]).cuda()
+    lse = torch.randn(n, h, l, generator=gen).cuda() * 0.1 + float(np.log(s))
+    lens = [s - (b * 31) % (s // 2) for b in range(g)]
+    lim = [[0] * l for _ in range(g)]
+    for b in range(g):
+        for t, i in enumerate(sorted(torch.randperm(l, generator=gen)[:max(2, l // 8)].tolist())):
+            lim[b][i] = lens[b] - 5 + t
+        lim[b][0], lim[b][l - 1], lim[b][l // 2], lim[b][l // 3] = 1, 1 << 40, -3, 128
+    if g > 2:
+        lim[2] = [0] * l
+    mass = torch.rand(n, hk, s, generator=gen).cuda()
+    out = _ffi.attn_mass(Q, K, lse, kv_lens=lens_t(lens), q_lens=lens_t(lim), mass=mass)
+    check_mass(Q, K, lse, lens * layers, lim * layers, mass, out)
+    assert torch.equal(out[0, :, lens[0]:], mass[0, :, lens[0]:])
+    if g > 2:
+        assert torch.equal(out[2::g], mass[2::g])
+    inplace = mass.clone()
+    _ffi.attn_mass(Q, K, lse, kv_lens=lens_t(lens), q_lens=lens_t(lim), mass=inplace, out=inplace)
+    assert torch.equal(inplace, out) and _ffi.tc_error() == 0
+    # the limits alone say how many entries share them
+    alone = _ffi.attn_mass(Q, K, lse, q_lens=lens_t(lim))
+    check_mass(Q, K, lse, [s] * n, lim * layers, None, alone)

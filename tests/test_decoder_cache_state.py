@@ -146,3 +146,29 @@ def test_a_window_of_no_prompt_rows(cuda):
     assert abs(float(dec.mass.sum()) - rows) < 2e-2 * rows
     with pytest.raises(ValueError):
         dec.alloc_cache(2, 16, track_mass=True, window=-1)
+
+
+@pytest.mark.gpu
+def test_right_drafts_take_fewer_steps(cuda):
+    """Drafts that are the model's own continuation are accepted: a generation with them takes a fraction of the steps."""
+    dec = _decoder(64, seed=5)
+    ids = torch.randint(0, 1000, (1, 12), generator=torch.Generator().manual_seed(6)).cuda()
+    plan, steps = TreePlan([-1, 0, 0, 1]), [0, 0]
+    dec.alloc_cache(1, 64)
+
+    def nothing(last, step):
+        steps[0] += 1
+        return torch.full((1, 3), 1001 - 2, dtype=torch.int64, device="cuda")
+    plain = dec.generate_tree(ids, 24, plan, nothing)
+
+    def helper(last, step):
+        steps[1] += 1
+        at = int(dec.next_pos[0]) - 12 if dec.kv_lens is not None else 0
+        nxt = plain[0, at + 1:at + 3].tolist() + [0, 0]
+        return torch.tensor([[nxt[0], 7, nxt[1]]], device="cuda")
+    dec.alloc_cache(1, 64)
+    helped = dec.generate_tree(ids, 24, plan, helper)
+    # the same rows in the same tree positions give the same logits, so nothing but the drafts differs
+    assert torch.equal(helped[0, :3], plain[0, :3])
+    same = int((helped[0] == plain[0]).int().cumprod(0).sum())
+    assert steps[0] >= 20 and steps[1] <= 8 + (24 - same), (steps, same)
