@@ -529,24 +529,30 @@ class Decoder:
     def generate_tree(self, ids, new_tokens, plan, propose, budget=None, sinks=4, recent=64):
         """Greedy decoding with drafts: propose(last [B], step) gives the drafted tokens [B, plan.size - 1] below each sequence's last
         token.  With a budget the cache is evicted down to it whenever the next step might not fit the capacity.  Returns the
-        generated ids [B, new_tokens], the same as greedy decoding without drafts (up to ties within rounding)."""
+        generated ids [B, new_tokens], the same as greedy decoding without drafts (up to ties within rounding).  Without one
+        a capacity of prompt + new_tokens - 1 + plan.max_depth is enough: a sequence that has its tokens takes no more slots."""
         last = self.next_token(self.prefill(ids, local_logits=True))
         out = [[int(t)] for t in last.tolist()]
-        used, step = ids.shape[1], 0
+        used, step = [ids.shape[1]] * ids.shape[0], 0           # slots in use per sequence
         while min(len(o) for o in out) < new_tokens:
-            if used + plan.max_depth > self.cap:
+            if max(used) + plan.max_depth > self.cap:
                 if budget is None:
                     raise ValueError("generate_tree: the cache is full; give it a budget")
                 self.evict(budget, sinks, recent)
-                used = min(used, budget)
-                if used + plan.max_depth > self.cap:
+                used = [min(u, budget) for u in used]
+                if max(used) + plan.max_depth > self.cap:
                     raise ValueError("generate_tree: a budget has to leave room for a step")
             tokens = torch.cat([last[:, None], propose(last, step)], 1) if plan.size > 1 else last[:, None]
             path, counts, nxt = self.verify(tokens.contiguous(), plan)
             said = torch.where(path >= 0, tokens.gather(1, path.clamp(min=0)), path)
-            for o, row, c, t in zip(out, said.tolist(), counts.tolist(), nxt.tolist()):
+            over = []                                           # tokens beyond those asked for: they leave the cache again
+            for b, (o, row, c, t) in enumerate(zip(out, said.tolist(), counts.tolist(), nxt.tolist())):
+                over.append(min(c, max(0, len(o) + c - new_tokens)))
+                used[b] += c - over[b]
                 o += row[1:c] + [t]
-            used += int(counts.max())
+            if any(over):
+                back = torch.tensor(over, dtype=torch.int64, device=self.device)
+                self.kv_lens, self.next_pos = self.kv_lens - back, self.next_pos - back
             last, step = nxt, step + 1
         return torch.tensor([o[:new_tokens] for o in out], dtype=torch.int64, device=self.device)
 

@@ -172,3 +172,26 @@ def test_right_drafts_take_fewer_steps(cuda):
     assert torch.equal(helped[0, :3], plain[0, :3])
     same = int((helped[0] == plain[0]).int().cumprod(0).sum())
     assert steps[0] >= 20 and steps[1] <= 8 + (24 - same), (steps, same)
+
+
+@pytest.mark.gpu
+def test_generation_with_uneven_drafts_fits_the_tokens_asked_for(cuda):
+    """One sequence's drafts are right and the other's are noise, in turns: neither what the two take together nor what the faster one
+    takes after its last token counts as slots in use."""
+    dec = _decoder(64, seed=5)
+    g = torch.Generator().manual_seed(6)
+    ids, plan, new = torch.randint(0, 1000, (2, 12), generator=g).cuda(), TreePlan.chain(3), 30
+    dec.alloc_cache(2, 64)
+    plain = dec.generate_tree(ids, new, TreePlan.chain(1), None)
+    enough = 12 + new - 1 + plan.max_depth
+    for helped in (lambda b, step: b == 0, lambda b, step: b == step % 2):
+        def propose(last, step):
+            rows = []
+            for b in range(2):
+                at = int(dec.next_pos[b]) - 12 if dec.kv_lens is not None else 0
+                rows.append((plain[b, at + 1:at + 3].tolist() + [0, 0])[:2] if helped(b, step) else [999, 999])
+            return torch.tensor(rows, device="cuda")
+        dec.alloc_cache(2, enough)
+        got = dec.generate_tree(ids, new, plan, propose)
+        assert got.shape == (2, new) and dec.kv_lens.tolist() == dec.next_pos.tolist() == [12 + new - 1] * 2
+        assert torch.equal(got[:, :4], plain[:, :4])
