@@ -278,6 +278,9 @@ def workspace(kind, device, nbytes):
     key = (kind, device.index if device.index is not None else torch.cuda.current_device(), _stream())
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
+        if kind in ("sdpa", "reduce") and _capturing():
+            # ticket words made in a capture are zeroed when its graph runs: no eager call and no other graph may count on that
+            return torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
         cap = max(int(nbytes), 1 << 20)
         buf = torch.zeros(cap, dtype=torch.uint8, device=device)
         _scratch[key] = buf

@@ -46,3 +46,48 @@ def test_calls_of_growing_batches_share_a_workspace(cuda, calls):
             assert torch.isfinite(out).all() and float((out.double() - want).abs().max()) <= tol[kind] * float(v.abs().max())
     stream.synchronize()
     assert _ffi.tc_error() == 0
+
+
+def test_a_workspace_made_inside_a_capture_stays_with_its_graph(monkeypatch):
+    """Memory of a capture holds zeros only once the graph has run: it is not kept for calls outside."""
+    dev = torch.device("cpu", 0)
+    monkeypatch.setattr(_ffi, "_stream", lambda: 12345)
+    monkeypatch.setattr(_ffi, "_scratch", {})
+    monkeypatch.setattr(_ffi, "_capturing", lambda: True)
+    first, second = _ffi.workspace("sdpa", dev, 5000), _ffi.workspace("sdpa", dev, 5000)
+    assert first.data_ptr() != second.data_ptr() and first.numel() >= 5000 and int(first.sum()) == 0 and not _ffi._scratch
+    monkeypatch.setattr(_ffi, "_capturing", lambda: False)
+    kept = _ffi.workspace("sdpa", dev, 5000)
+    assert kept.data_ptr() == _ffi.workspace("sdpa", dev, 7000).data_ptr()
+    monkeypatch.setattr(_ffi, "_capturing", lambda: True)
+    assert _ffi.workspace("sdpa", dev, 5000).data_ptr() == kept.data_ptr()          # made before: zero already
+    assert _ffi.workspace("sdpa", dev, 2 << 20).data_ptr() != kept.data_ptr() and len(_ffi._scratch) == 1
+
+
+@pytest.mark.gpu
+def test_attention_first_called_inside_a_capture(cuda):
+    """Split attention captured on a fresh stream without a warm-up, replayed, and called eagerly on that stream before and after."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(2, hh, ll, 128, generator=g, device="cuda").bfloat16() for hh, ll in ((16, 1), (8, 4096), (8, 4096)))
+    want = _want(q, k, v)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        outs = [_ffi.sdpa(q, k, v)[0] for _ in range(3)]
+
+    def eager():
+        with torch.cuda.stream(side):
+            out = torch.full((2, 16, 1, 128), float("nan"), device="cuda", dtype=torch.bfloat16)
+            return _ffi.sdpa(q, k, v, out=out)[0]
+    got = [eager()]
+    for _ in range(3):
+        for out in outs:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got += [eager()] + [out.clone() for out in outs]
+    torch.cuda.synchronize()
+    for out in got:
+        assert torch.isfinite(out).all() and float((out.double() - want).abs().max()) <= 3 * 2.0 ** -8 * float(v.abs().max())
+    del graph
