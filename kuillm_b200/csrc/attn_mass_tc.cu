@@ -14,7 +14,10 @@
 //   stream past a resident K tile (128 columns: a 64-column product would be bound by shared memory, whose A operand it reads
 //   twice as often) and every group takes 32 columns of each.  Items are dealt in alternating direction, which evens out a causal mask's
 //   falling work per item.  (Making a quarter of the exponentials by a polynomial in the FMA pipe was slower, 396 against
-//   361 us for an 8192-token prompt, which now takes 323 us: the instructions it takes are what the scheduler has least of.)
+//   361 us for an 8192-token prompt, which now takes 323 us at 1965 MHz: the instructions it takes are what the scheduler has least of.)
+//
+// Weights and their sums stay in 32 bits.  Beside its score a weight is off by the special-function unit's 2^-22 and by the rounding of
+// lse to the log2 domain, 2^-24 |lse|.
 #include "tree.cuh"
 #include "tc_ptx.cuh"
 #include <type_traits>

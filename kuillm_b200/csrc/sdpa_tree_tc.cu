@@ -6,8 +6,9 @@
 // A segment that is a whole unit writes its rows; the others leave records, which a second kernel joins.  (Joining them in the CTA
 // that finishes a unit last was slower, 87 against 69 us for 16 x 27 rows over 4096 keys: four warps cannot hide it.)  Rows beyond 128
 // per unit (G heads x lt drafted positions, one TMA box) go to further CTAs with the same range, which find the tiles in L2.
-// 32 / 8 heads of 128: 16 sequences x 27 rows over 2000 to 4001 keys 63 us (the stream alone 39 us, 5 TB/s); 2 x 64 rows over 65000 keys 170 us,
-// bound by the second row tile's passage through L2; 8 rows over 517 keys 12.5 us, launches and set-up.
+// 32 / 8 heads of 128, replayed at 1965 MHz: 16 sequences x 27 rows over 2000 to 4001 keys 64 us (the stream alone 39 us, 5 TB/s); 2 x 64 rows
+// over 65000 keys 171 us, where no unit is busy for more than a third of the time (counted over 16000 keys: tensor 28 %, special functions
+// 29 %, L2 24 %, DRAM 30 %) and each tile's chain from scores to product is what is waited for; 8 rows over 517 keys 12.7 us, the set-up of two launches.
 //
 // K and V tiles arrive through one in-order TMA ring (K0 V0 K1 V1 ...); S = Q K^T goes to TMEM (double buffered), the softmax
 // is online with one thread per row, P returns to TMEM over the scores it came from and is the A operand of O += P V.  Two
@@ -522,6 +523,10 @@ sdpa_tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             tc::tmem_st_wait();
           }
         }
+        // The weights are rounded to the element type here (by half a step at most: 2^-8 of a weight in bf16, 2^-11 in fp16): the product takes both operands
+        // in one type, and kuiops_sdpa does the same.  Their sum is taken before.  Against the definition in 64 bits a bf16 result
+        // is off by 0.0018 to 0.0021 of its norm where rounding the result alone costs 0.0016 to 0.0017.  A second product with what the
+        // rounding left off brings that back, but takes 4 % longer for 16 x 27 rows over 4000 keys and 21 % for 2 x 64 over 65000.
         // P over the scores it came from: column c holds keys 2 c and 2 c + 1, zero outside this copy's columns
         const uint32_t p_addr = tmem_S + (g & 1) * RTN + lane_addr;
         if constexpr (REP == 1) {
