@@ -389,7 +389,8 @@ KUIOPS_API int kuiops_sdpa_noalloc(int dtype, uint32_t n, uint32_t h, uint32_t h
  * views of the packed projection rows kuiops_rope_qkv leaves.  mask is bytes, l x l per entry, with strides for (entry,
  * row, key); mask_sn = 0: one mask for all.  A key that a row does not see takes no part in it, whatever its
  * rows hold (infinities, NaN); a row that sees no key gives 0 and -inf.  A value that is not finite reaches the rows that see it
- * as in a sum with positive weights: an infinity, or NaN where both signs or a NaN meet.  fp32 accumulation; 16-bit types round the
+ * as in a sum with positive weights: an infinity, or NaN where both signs or a NaN meet (and where its weight, relative to the row's
+ * largest, is below the least that fp32 holds).  fp32 accumulation; 16-bit types round the
  * softmax weights to the element type before the product with V, as kuiops_sdpa does.
  * s may be 0 (K and V may then be NULL).  e <= 1024, ev <= 256 (KUIOPS_EUNSUPPORTED beyond),
  * l <= KUIOPS_TREE_MAX_ROWS.  workspace: kuiops_sdpa_tree_workspace_bytes(...) bytes, 16-byte aligned, no initial
